@@ -48,6 +48,11 @@ SIGNATURES = {
   "cdb_fp8_gemm_plan": (c_int, [c_void_p, c_int, c_int, c_void_p, c_void_p]),
   "cdb_tuning_set_gemm_tile_cols": (c_int, [c_int]),
   "cdb_tuning_set_gemm_kernel": (c_int, [c_int]),
+  "cdb_fp4_block_scale_bytes": (c_size_t, [c_int64, c_int64, c_int]),
+  "cdb_fp4_quant_rows": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p]),
+  "cdb_fp4_dequant_rows": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int, c_void_p, c_int, c_void_p]),
+  "cdb_fp4_gemm": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int, c_int, c_int,
+                           c_void_p, c_void_p]),
   "cdb_qk_norm_rope": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64,
                                c_int64, c_int64, c_int, c_int, c_int, c_float, c_void_p]),
   "cdb_gated_residual_pair": (c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64,
@@ -273,7 +278,8 @@ def release_peer_sync(device):
 def raise_on_device_status(gemm_status: int, peer_status: int):
   """Turn the latched status words (host copies) into the C ABI's CDB_ERR_DEVICE_TIMEOUT as an exception."""
   if gemm_status != 0:
-    raise DeviceTimeoutError(f"CDB_ERR_DEVICE_TIMEOUT: a bounded wait inside the FP8 GEMM ran out (code {gemm_status}); "
+    which = "FP8 GEMM" if gemm_status < 20 else "4-bit product" if gemm_status < 30 else "cross attention"
+    raise DeviceTimeoutError(f"CDB_ERR_DEVICE_TIMEOUT: a bounded wait inside the {which} ran out (code {gemm_status}); "
                              "the products launched since are incomplete")
   if peer_status != 0:
     raise DeviceTimeoutError(f"CDB_ERR_DEVICE_TIMEOUT: the signal of peer {peer_status - 1} did not arrive within the "
@@ -651,3 +657,47 @@ def gated_residual_pair(xa, gate_a, ya, xb, gate_b, yb):
   st = lib().cdb_gated_residual_pair(*args, cols, _stream(xa))
   check(st, "cdb_gated_residual_pair")
   return outs[0], outs[1]
+
+
+# ---- 4-bit microscaled matrices ------------------------------------------------------------------
+FP4_FORMATS = {"nvfp4": 0, "mxfp4": 1}
+FP4_BLOCK = {"nvfp4": 16, "mxfp4": 32}
+FP4_MAX_COLS = 16384
+
+
+class Fp4Matrix(ctypes.Structure):
+  """ctypes image of `cdb_fp4_matrix`."""
+  _fields_ = [("codes", c_void_p), ("block_scales", c_void_p), ("row_scale", c_void_p)]
+
+
+def fp4_block_scale_bytes(rows: int, cols: int, fmt: str) -> int:
+  """Bytes of the tiled block scales of a [rows, cols] matrix (host arithmetic only)."""
+  tiles = -(-cols // 256) * (256 // FP4_BLOCK[fmt]) // 4
+  return -(-rows // 128) * tiles * 512
+
+
+def fp4_quant_rows(x2d, codes, block_scales, row_scale, fmt: str):
+  """x2d [rows, cols] f32 / bf16 / f16 (rows may be strided) -> 4-bit codes and scales (see cdb_fp4_quant_rows)."""
+  rows, cols = x2d.shape
+  with torch.cuda.device(x2d.device):
+    st = lib().cdb_fp4_quant_rows(_ptr(x2d), rows, cols, x2d.stride(0) if rows > 1 else cols, DTYPE_ID[x2d.dtype],
+                                  FP4_FORMATS[fmt], _ptr(codes), _ptr(block_scales), _ptr(row_scale), _stream(x2d))
+  check(st, "cdb_fp4_quant_rows")
+
+
+def fp4_dequant_rows(codes, block_scales, row_scale, cols: int, fmt: str, out):
+  with torch.cuda.device(out.device):
+    st = lib().cdb_fp4_dequant_rows(_ptr(codes), _ptr(block_scales), _ptr(row_scale), out.shape[0], cols, FP4_FORMATS[fmt],
+                                    _ptr(out), DTYPE_ID[out.dtype], _stream(out))
+  check(st, "cdb_fp4_dequant_rows")
+
+
+def fp4_gemm(a, w, bias, out, cols: int, fmt: str, gelu: bool = False):
+  """out [M, N] = act(a [M, cols] @ w [N, cols]^T + bias) for two (codes, block_scales, row_scale) triples (see cdb_fp4_gemm)."""
+  M, N = out.shape
+  am, wm = (Fp4Matrix(*[None if t is None else t.data_ptr() for t in triple]) for triple in (a, w))
+  with torch.cuda.device(out.device):
+    st = lib().cdb_fp4_gemm(ctypes.byref(am), ctypes.byref(wm), _ptr(bias), _ptr(out), M, N, cols,
+                            out.stride(0) if M > 1 else N, FP4_FORMATS[fmt], DTYPE_ID[out.dtype], int(gelu),
+                            _ptr(gemm_status_word(out.device)), _stream(out))
+  check(st, "cdb_fp4_gemm")

@@ -1,0 +1,733 @@
+// 4-bit microscaled product for sm_100a: out[m, n] = act(sum_k A[m, k] W[n, k] + bias[n])  (formats: fp4.cuh)
+//
+// The tensor core multiplies the e2m1 codes and applies both operands' block scales itself (tcgen05.mma with
+// .block_scale, K = 64 per instruction), so the sum over all blocks stays one fp32 accumulation in tensor memory; the
+// row scales of nvfp4, the bias and the optional tanh-GELU are applied in the epilogue.
+//
+//   * operands and their block scales by TMA into a ring of shared-memory stages of 256 columns (128 bytes) of K;
+//     block scales go on to tensor memory (tcgen05.cp, 32 rows x 16 bytes broadcast to the four lane quarters);
+//   * CG = 2: a pair of SMs works on a 256 x bn tile (each CTA loads 128 rows of A, half of the weight tile, and the
+//     weight tile's scales whole, since each tensor core needs them); CG = 1: one SM, 128 x bn;
+//   * two accumulators in tensor memory, so that a tile's epilogue overlaps the next tile's main loop.  Two of 256
+//     columns leave no room for the scales (512 columns in all): at bn = 256 the second starts at column 160 and the
+//     two share 96 columns.  The epilogue reads those 96 columns into registers first and hands them over; all that
+//     the next tile's MMAs wait for is that read.
+//   * M <= 4 rows: no tile; the weights are streamed once by the CUDA cores (fp4_gemv_kernel).
+//
+// Warp roles (192 threads): warp 0 = TMA producer, warp 1 = tensor memory owner and MMA issuer, warps 2..5 = epilogue.
+// Every wait is bounded (bounded_wait): on expiry the roles drain, tensor memory is freed and the kernel returns.
+#include <cuda_fp16.h>
+
+#include <cstdlib>
+
+#include "fp4.cuh"
+#include "tcgen05.cuh"
+
+namespace cdb {
+
+constexpr int F4_THREADS = 192;
+constexpr int F4_EPI_WARP0 = 2;
+constexpr int F4_EPI_THREADS = 128;
+constexpr int F4_MAX_STAGES = 8;
+constexpr int F4_MAX_BN = 256;
+constexpr int F4_A_BYTES = 128 * 128;     // 128 rows of one step's codes
+constexpr uint32_t F4_TMEM_COLS = 512;
+constexpr uint32_t F4_SHARED_COL = 160;   // where the second accumulator starts when bn = 256
+constexpr uint32_t F4_SF_COL = 416;       // scales: two slots of 48 columns (16 for A, 32 for W)
+constexpr uint32_t F4_SF_SLOT = 48;
+constexpr int F4_BLOCK_BYTES = 32 * 64 * 2;                      // one staged block of output: 32 rows x 64 columns
+constexpr int F4_STAGING_BYTES = (F4_EPI_THREADS / 32) * 2 * F4_BLOCK_BYTES;
+constexpr int F4_SMEM_LIMIT = 232448;
+
+struct __align__(8) F4Barriers {
+  uint64_t full[F4_MAX_STAGES];
+  uint64_t empty[F4_MAX_STAGES];
+  uint64_t acc_full[2];
+  uint64_t acc_empty[2];
+  uint32_t tmem_base;
+  volatile int abort_flag;
+};
+constexpr int F4_FIXED_BYTES = 1024 + F4_STAGING_BYTES + F4_MAX_BN * 8 + (int)sizeof(F4Barriers);
+
+struct F4Params {
+  CUtensorMap map_a, map_w, map_sa, map_sw, map_out;
+  const float* ra;  // row scales, or null (mxfp4)
+  const float* rw;
+  const void* bias;
+  int M, N;
+  int m_tiles, n_tiles, k_steps, group_m, num_tiles;
+  int bn, stages, stage_bytes, gelu;
+  uint32_t idesc;
+};
+
+__device__ __forceinline__ void tma_load_3d(const CUtensorMap* map, uint64_t* bar, void* dst, int c0, int c1, int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+      ::"r"(smem_u32(dst)), "l"(map), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_3d_pair(const CUtensorMap* map, uint32_t bar_cluster_addr, void* dst, int c0,
+                                                 int c1, int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+      ::"r"(smem_u32(dst)), "l"(map), "r"(bar_cluster_addr), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
+// 32 rows x 16 bytes of shared memory -> 4 tensor memory columns, the same in all four lane quarters (CG = 2: in both
+// CTAs, each from its own shared memory).
+template <int CG>
+__device__ __forceinline__ void copy_scales(uint32_t tmem, uint64_t desc) {
+  if constexpr (CG == 2) asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+  else asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+}
+#define CDB_F4_MMA(CG_, KIND_)                                                                                  \
+  asm volatile(                                                                                                 \
+      "{\n\t.reg .pred p;\n\t"                                                                                  \
+      "setp.ne.b32 p, %6, 0;\n\t"                                                                               \
+      "tcgen05.mma.cta_group::" CG_ ".kind::" KIND_ " [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(tmem_d),      \
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)                                    \
+      : "memory")
+template <int CG, bool NV>
+__device__ __forceinline__ void mma_f4(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t sfa,
+                                       uint32_t sfb, uint32_t accumulate) {
+  if constexpr (CG == 1 && NV) CDB_F4_MMA("1", "mxf4nvf4.block_scale.scale_vec::4X");
+  if constexpr (CG == 1 && !NV) CDB_F4_MMA("1", "mxf4.block_scale.scale_vec::2X");
+  if constexpr (CG == 2 && NV) CDB_F4_MMA("2", "mxf4nvf4.block_scale.scale_vec::4X");
+  if constexpr (CG == 2 && !NV) CDB_F4_MMA("2", "mxf4.block_scale.scale_vec::2X");
+}
+// Block-scaled instruction descriptor: [4,6) scale id of B, [7,10) A = e2m1 (1), [10,13) B = e2m1 (1), [17,23) N >> 3,
+// bit 23 scale type (0 = e4m3, 1 = e8m0), [24,29) M >> 4, [29,31) scale id of A.  The scale id picks the half of a
+// tensor memory word that holds an instruction's two e8m0 scales (0 or 2).
+constexpr uint32_t f4_idesc(int m, int n, bool nv) {
+  return (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((nv ? 0u : 1u) << 23) | ((uint32_t)(m >> 4) << 24);
+}
+// Descriptor of one 512-byte scale tile: no swizzle, groups of 8 rows x 16 bytes 128 bytes apart.
+__device__ __forceinline__ uint64_t scale_tile_desc(uint32_t smem_addr) {
+  return (uint64_t)((smem_addr & 0x3FFFFu) >> 4) | ((uint64_t)(128 >> 4) << 16) | ((uint64_t)(128 >> 4) << 32) | ((uint64_t)1 << 46);
+}
+// M fastest inside groups of `group_m` row tiles, so a wave shares weight tiles and a bounded set of A panels in L2.
+__device__ __forceinline__ void f4_tile_coords(int tile, const F4Params& p, int& mi, int& ni) {
+  const int per_group = p.group_m * p.n_tiles;
+  const int group = tile / per_group;
+  const int first_m = group * p.group_m;
+  const int rows = min(p.group_m, p.m_tiles - first_m);
+  const int in_group = tile - group * per_group;
+  mi = first_m + in_group % rows;
+  ni = in_group / rows;
+}
+__device__ __forceinline__ bool f4_epi_all(bool pred) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %1, 0;\n\t"
+      "bar.red.and.pred q, 1, %2, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"((uint32_t)pred), "n"(F4_EPI_THREADS)
+      : "memory");
+  return r != 0;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (__is_same(T, __nv_bfloat16)) {
+    return pack_bf16x2(lo, hi);
+  } else {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+}
+
+// One staged block: 32 rows x 64 columns starting at local column `c0` of the tile, from 2 x 32 accumulator registers.
+template <typename T>
+__device__ __forceinline__ void f4_store_block(const F4Params& p, uint8_t* staging, uint32_t& blocks_done,
+                                               const uint32_t (&lo)[32], const uint32_t (&hi)[32], int c0, int n0,
+                                               int row0, float rs, const float2* s_col, int lane) {
+  if (n0 + c0 >= p.N) return;
+  uint8_t* block = staging + (blocks_done & 1u) * F4_BLOCK_BYTES;
+  if (lane == 0) bulk_wait_group_read<1>();  // the store that used this block two blocks ago is done reading
+  __syncwarp();
+  uint8_t* rowp = block + lane * 128;
+#pragma unroll
+  for (int g = 0; g < 8; ++g) {  // 8 columns = one 16-byte chunk
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int c = g * 8 + 2 * j;
+      const float4 sb = *reinterpret_cast<const float4*>(s_col + c0 + c);  // (scale, bias) of two columns
+      const float a0 = __uint_as_float(c < 32 ? lo[c & 31] : hi[c & 31]);
+      const float a1 = __uint_as_float(c < 32 ? lo[(c + 1) & 31] : hi[(c + 1) & 31]);
+      float v0 = fmaf(a0 * rs, sb.x, sb.y), v1 = fmaf(a1 * rs, sb.z, sb.w);
+      if (p.gelu) {
+        v0 = gelu_tanh(v0);
+        v1 = gelu_tanh(v1);
+      }
+      w[j] = pack2<T>(v0, v1);
+    }
+    *reinterpret_cast<uint4*>(rowp + ((g ^ (lane & 7)) * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  fence_async_smem();
+  __syncwarp();
+  if (lane == 0) {
+    tma_store_2d(&p.map_out, block, n0 + c0, row0);
+    bulk_commit_group();
+  }
+  ++blocks_done;
+}
+
+template <int CG, bool NV, typename T>
+__global__ void __launch_bounds__(F4_THREADS, 1) fp4_gemm_kernel(const __grid_constant__ F4Params p, int32_t* status_word) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  uint8_t* s_staging = smem + p.stages * p.stage_bytes;  // a multiple of 1024
+  float2* s_col = reinterpret_cast<float2*>(s_staging + F4_STAGING_BYTES);
+  F4Barriers* gb = reinterpret_cast<F4Barriers*>(s_col + F4_MAX_BN);
+
+  constexpr int TILES = NV ? 4 : 2;  // scale tiles of one step and panel
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const uint32_t rank = CG == 2 ? cluster_ctarank() : 0u;  // 0 owns the shared barriers and issues the MMAs
+  const int first = CG == 2 ? blockIdx.x >> 1 : blockIdx.x;
+  const int step = CG == 2 ? gridDim.x >> 1 : gridDim.x;
+  const int bn = p.bn;
+  const int panels = bn > 128 ? bn / 128 : 1;
+  const uint32_t b_bytes = (uint32_t)(CG == 2 ? bn >> 1 : bn) * 128u;
+  const uint32_t sfa_off = F4_A_BYTES + b_bytes;
+  const uint32_t sfb_off = sfa_off + TILES * 512;
+  const bool shared_acc = bn == F4_MAX_BN;
+  const uint32_t acc1 = shared_acc ? F4_SHARED_COL : (uint32_t)bn;
+  const int stages = p.stages;
+  pdl_launch_dependents();
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < F4_MAX_STAGES; ++s) {
+      mbar_init(&gb->full[s], 1);
+      mbar_init(&gb->empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&gb->acc_full[b], 1);
+      mbar_init(&gb->acc_empty[b], CG * (F4_EPI_THREADS / 32));
+    }
+    gb->abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    if constexpr (CG == 2) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&gb->tmem_base)), "r"(F4_TMEM_COLS) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&gb->tmem_base)), "r"(F4_TMEM_COLS) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  if constexpr (CG == 2) cluster_sync_all();  // the peer's barriers exist before anything is signalled across the pair
+  tcgen05_fence_after();
+  const uint32_t tmem_base = gb->tmem_base;
+
+  if (warp == 0) {
+    // ---------------- TMA producer ----------------
+    if (lane == 0) {
+      uint32_t it = 0;
+      bool ok = true;
+      const uint32_t tx = CG * (sfb_off + (uint32_t)panels * TILES * 512);  // both CTAs' bytes of one stage
+      for (int tile = first; tile < p.num_tiles && ok; tile += step) {
+        int mi, ni;
+        f4_tile_coords(tile, p, mi, ni);
+        const int m0 = mi * (128 * CG) + (int)rank * 128;
+        const int n0 = ni * bn;
+        const int w0 = n0 + (CG == 2 ? (int)rank * (bn >> 1) : 0);
+        for (int kb = 0; kb < p.k_steps; ++kb, ++it) {
+          const int s = it % stages;
+          ok = bounded_wait(&gb->empty[s], ((it / stages) & 1u) ^ 1u, &gb->abort_flag, status_word, 21);
+          if (!ok) break;
+          uint8_t* dst = smem + s * p.stage_bytes;
+          if constexpr (CG == 2) {
+            if (rank == 0) mbar_expect_tx(&gb->full[s], tx);
+            const uint32_t full = map_to_cta(smem_u32(&gb->full[s]), 0);
+            tma_load_2d_pair(&p.map_a, full, dst, kb * 128, m0);
+            tma_load_2d_pair(&p.map_w, full, dst + F4_A_BYTES, kb * 128, w0);
+            tma_load_3d_pair(&p.map_sa, full, dst + sfa_off, 0, kb * TILES * 4, m0 >> 7);
+            tma_load_3d_pair(&p.map_sw, full, dst + sfb_off, 0, kb * TILES * 4, n0 >> 7);
+          } else {
+            mbar_expect_tx(&gb->full[s], tx);
+            tma_load_2d(&p.map_a, &gb->full[s], dst, kb * 128, m0);
+            tma_load_2d(&p.map_w, &gb->full[s], dst + F4_A_BYTES, kb * 128, w0);
+            tma_load_3d(&p.map_sa, &gb->full[s], dst + sfa_off, 0, kb * TILES * 4, m0 >> 7);
+            tma_load_3d(&p.map_sw, &gb->full[s], dst + sfb_off, 0, kb * TILES * 4, n0 >> 7);
+          }
+        }
+      }
+      // A CTA may not retire while copies into its shared memory are in flight or while MMAs read it: wait (bounded,
+      // also after an abort) until the MMAs released every stage used.
+      const uint64_t t0 = global_timer_ns();
+      for (uint32_t j = (it > (uint32_t)stages ? it - stages : 0); j < it; ++j) {
+        while (!mbar_try_wait(&gb->empty[j % stages], (j / stages) & 1u)) {
+          if (global_timer_ns() - t0 > BARRIER_LIMIT_NS) break;
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ---------------- MMA issuer ----------------
+    if (lane == 0 && rank == 0) {
+      uint32_t it = 0, n_tile = 0;
+      bool ok = true;
+      for (int tile = first; tile < p.num_tiles && ok; tile += step, ++n_tile) {
+        const uint32_t buf = n_tile & 1u;
+        // Separate accumulators: tile n_tile - 2 has left this one.  Shared columns: tile n_tile - 1 has left them
+        // (and n_tile - 2 everything, since the epilogue takes tiles in order).
+        if (!shared_acc) {
+          ok = bounded_wait(&gb->acc_empty[buf], ((n_tile >> 1) & 1u) ^ 1u, &gb->abort_flag, status_word, 22);
+        } else if (n_tile > 0) {
+          ok = bounded_wait(&gb->acc_empty[buf ^ 1u], ((n_tile - 1) >> 1) & 1u, &gb->abort_flag, status_word, 22);
+        }
+        if (!ok) break;
+        tcgen05_fence_after();
+        const uint32_t tmem_d = tmem_base + buf * acc1;
+        int mi, ni;
+        f4_tile_coords(tile, p, mi, ni);
+        // a 64-column tile may be the second half of its panel of 128 weight rows: scales two columns on
+        const uint32_t sfb_skip = (uint32_t)((ni * bn) & 127) >> 5;
+        for (int kb = 0; kb < p.k_steps; ++kb, ++it) {
+          const int s = it % stages;
+          ok = bounded_wait(&gb->full[s], (it / stages) & 1u, &gb->abort_flag, status_word, 23);
+          if (!ok) break;
+          // The scale slot of this step was read by the MMAs of step it - 2: they have retired when their stage is
+          // released.  The MMAs of step it - 1 are still queued, so the tensor pipe does not run dry meanwhile.
+          if (it >= 2) {
+            const uint32_t u = it - 2;
+            ok = bounded_wait(&gb->empty[u % stages], (u / stages) & 1u, &gb->abort_flag, status_word, 24);
+            if (!ok) break;
+          }
+          tcgen05_fence_after();
+          const uint32_t base = smem_u32(smem + s * p.stage_bytes);
+          const uint32_t sfa = tmem_base + F4_SF_COL + (it & 1u) * F4_SF_SLOT;
+          const uint32_t sfb = sfa + 16;
+#pragma unroll
+          for (int j = 0; j < TILES; ++j) {
+            copy_scales<CG>(sfa + j * 4, scale_tile_desc(base + sfa_off + j * 512));
+            for (int q = 0; q < panels; ++q)
+              copy_scales<CG>(sfb + (j * panels + q) * 4, scale_tile_desc(base + sfb_off + (q * TILES + j) * 512));
+          }
+          const uint64_t adesc = make_kmajor_sw128_desc(base);
+          const uint64_t bdesc = make_kmajor_sw128_desc(base + F4_A_BYTES);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {  // 64 columns = 32 bytes: +2 in the (address >> 4) field
+            const int j = NV ? k : k >> 1;
+            const uint32_t id = NV ? 0u : (uint32_t)(k & 1) * 2u;
+            mma_f4<CG, NV>(tmem_d, adesc + 2 * k, bdesc + 2 * k, p.idesc | (id << 4) | (id << 29), sfa + j * 4,
+                           sfb + j * panels * 4 + sfb_skip, (kb | k) != 0 ? 1u : 0u);
+          }
+          if constexpr (CG == 2) tcgen05_commit_both(smem_u32(&gb->empty[s]));
+          else tcgen05_commit(&gb->empty[s]);
+        }
+        if (ok) {
+          if constexpr (CG == 2) tcgen05_commit_both(smem_u32(&gb->acc_full[buf]));
+          else tcgen05_commit(&gb->acc_full[buf]);
+        }
+      }
+    }
+    __syncwarp();
+  } else {
+    // ---------------- epilogue: this CTA's 128 rows x bn columns ----------------
+    const int quarter = warp & 3;
+    const int et = threadIdx.x - F4_EPI_WARP0 * 32;
+    uint8_t* staging = s_staging + quarter * 2 * F4_BLOCK_BYTES;
+    const T* bias = static_cast<const T*>(p.bias);
+    uint32_t n_tile = 0, blocks_done = 0;
+    bool ok = true;
+    for (int tile = first; tile < p.num_tiles && ok; tile += step, ++n_tile) {
+      int mi, ni;
+      f4_tile_coords(tile, p, mi, ni);
+      const int row0 = mi * (128 * CG) + (int)rank * 128 + quarter * 32;
+      const int n0 = ni * bn;
+      const uint32_t buf = n_tile & 1u;
+      asm volatile("bar.sync 1, %0;" ::"n"(F4_EPI_THREADS) : "memory");  // the last tile's readers of s_col are done
+      for (int c = et; c < bn; c += F4_EPI_THREADS) {
+        const int col = n0 + c;
+        float2 v = make_float2(0.f, 0.f);
+        if (col < p.N) {
+          v.x = p.rw != nullptr ? __ldg(p.rw + col) : 1.f;
+          if (bias != nullptr) v.y = (float)bias[col];
+        }
+        s_col[c] = v;
+      }
+      ok = bounded_wait(&gb->acc_full[buf], (n_tile >> 1) & 1u, &gb->abort_flag, status_word, 25);
+      ok = f4_epi_all(ok);  // publishes s_col, and makes the decision to go on the same in all four warps
+      if (!ok) break;
+      tcgen05_fence_after();
+      const int row = row0 + lane;
+      const float rs = row < p.M ? (p.ra != nullptr ? __ldg(p.ra + row) : 1.f) : 0.f;
+      const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + buf * acc1;
+      const bool live = row0 < p.M;  // warp-uniform: some of the 32 rows exist
+      auto release = [&] {
+        tcgen05_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if constexpr (CG == 2) mbar_arrive_cluster(map_to_cta(smem_u32(&gb->acc_empty[buf]), 0));
+          else mbar_arrive(&gb->acc_empty[buf]);
+        }
+      };
+      auto plain_blocks = [&](int from, int to) {
+#pragma unroll 1
+        for (int c = from; c < to && n0 + c < p.N; c += 64) {
+          uint32_t lo[32], hi[32];
+          tmem_ld_32x32b_x32(taddr + c, lo);
+          tmem_ld_32x32b_x32(taddr + c + 32, hi);
+          tmem_ld_wait();
+          f4_store_block<T>(p, staging, blocks_done, lo, hi, c, n0, row0, rs, s_col, lane);
+        }
+      };
+      if (!shared_acc) {
+        if (live) plain_blocks(0, bn);
+        release();
+      } else if (!live) {
+        release();
+      } else {
+        // the columns that the other accumulator overlaps: 160..255 of the first, 0..95 of the second
+        uint32_t s0[32], s1[32], s2[32], x[32];
+        const uint32_t at = taddr + (buf == 0 ? F4_SHARED_COL : 0u);
+        tmem_ld_32x32b_x32(at, s0);
+        tmem_ld_32x32b_x32(at + 32, s1);
+        tmem_ld_32x32b_x32(at + 64, s2);
+        tmem_ld_wait();
+        release();
+        if (buf == 0) {
+          f4_store_block<T>(p, staging, blocks_done, s1, s2, 192, n0, row0, rs, s_col, lane);
+          tmem_ld_32x32b_x32(taddr + 128, x);
+          tmem_ld_wait();
+          f4_store_block<T>(p, staging, blocks_done, x, s0, 128, n0, row0, rs, s_col, lane);
+          plain_blocks(0, 128);
+        } else {
+          f4_store_block<T>(p, staging, blocks_done, s0, s1, 0, n0, row0, rs, s_col, lane);
+          tmem_ld_32x32b_x32(taddr + 96, x);
+          tmem_ld_wait();
+          f4_store_block<T>(p, staging, blocks_done, s2, x, 64, n0, row0, rs, s_col, lane);
+          plain_blocks(128, 256);
+        }
+        tcgen05_fence_before();  // orders these reads before the next barrier, behind which MMAs may overwrite them
+      }
+    }
+    if (lane == 0) bulk_wait_group_all();
+    __syncwarp();
+  }
+
+  tcgen05_fence_before();
+  __syncthreads();
+  if constexpr (CG == 2) cluster_sync_all();  // neither CTA leaves while the other may still touch its memory
+  if (warp == 1) {
+    tcgen05_fence_after();
+    if constexpr (CG == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(F4_TMEM_COLS) : "memory");
+    else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(F4_TMEM_COLS) : "memory");
+  }
+}
+
+// ---- few rows -----------------------------------------------------------------------------------------------
+// M <= 4: a 128-row tile would be padding, and the weights (N * K * 9/16 bytes) are all there is to read.  A warp owns
+// the four columns n, n + 32, n + 64, n + 96 whose block scales share 16 bytes; a lane takes 64 columns of K at a time:
+// 32 bytes of codes of each, one 16-byte load of scales, and the activations, from shared memory, once for all four.
+// The sixteen products of a block are multiples of 0.25 and at most 36: eight of them sum exactly in f16 (at most 288),
+// so the two halves of a packed f16 accumulator hold a block's sum exactly; blocks are summed in fp32.
+constexpr int F4V_THREADS = 256;
+constexpr int F4V_MAX_M = 4;
+constexpr int F4V_SMEM_LIMIT = 96 * 1024;
+__host__ __device__ constexpr int f4v_row_bytes(int pieces) { return pieces * (128 + 16); }  // f16 codes and 4 fp32 scales
+
+template <bool NV>
+__device__ __forceinline__ void piece_scales(uint32_t word, int c, float (&s)[4]) {  // of the blocks of 16 of a piece
+  if constexpr (NV) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[i] = e4m3_to_float((word >> (8 * i)) & 0xffu);
+  } else {
+    word >>= (c & 1) * 16;
+    s[0] = s[1] = e8m0_to_float(word & 0xffu);
+    s[2] = s[3] = e8m0_to_float((word >> 8) & 0xffu);
+  }
+}
+
+template <int TM, bool NV, typename T>
+__global__ void __launch_bounds__(F4V_THREADS)
+    fp4_gemv_kernel(const uint8_t* __restrict__ a_codes, const uint8_t* __restrict__ a_scales, const float* __restrict__ ra,
+                    const uint8_t* __restrict__ w_codes, const uint8_t* __restrict__ w_scales, const float* __restrict__ rw,
+                    const T* __restrict__ bias, T* __restrict__ out, int64_t ld_out, int N, int K, int gelu) {
+  pdl_launch_dependents();
+  pdl_wait_prior();
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  const int pieces = (K + 63) >> 6;  // of 64 columns; the last may be half
+  const int chunks = K >> 5;         // of 32 columns = 16 bytes of codes
+  const int64_t tiles = fp4_panel_tiles(K, NV);
+  uint4* s_a = reinterpret_cast<uint4*>(smem_raw);                         // [TM][8][pieces]: 8 f16 codes each
+  float4* s_s = reinterpret_cast<float4*>(s_a + (size_t)TM * 8 * pieces);  // [TM][pieces]: scales of its 4 blocks of 16
+  for (int i = threadIdx.x; i < TM * pieces * 2; i += F4V_THREADS) {  // i = (m, piece, half)
+    const int m = i / (2 * pieces), h = i - m * 2 * pieces, c = h >> 1, half = h & 1;
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (h < chunks) v = *(reinterpret_cast<const uint4*>(a_codes + (int64_t)m * (K >> 1)) + h);
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint32_t f[4];
+      e2m1x8_to_half2(w[j], f);
+      s_a[(m * 8 + half * 4 + j) * pieces + c] = make_uint4(f[0], f[1], f[2], f[3]);
+    }
+    if (half == 0) {
+      const uint32_t word = *reinterpret_cast<const uint32_t*>(a_scales + fp4_scale_word(m, NV ? c : c >> 1, tiles));
+      float s[4];
+      piece_scales<NV>(word, c, s);
+      s_s[m * pieces + c] = make_float4(s[0], s[1], s[2], s[3]);
+    }
+  }
+  __syncthreads();
+  const int lane = threadIdx.x & 31;
+  const int warp = (blockIdx.x * F4V_THREADS + threadIdx.x) >> 5;
+  const int nwarps = (gridDim.x * F4V_THREADS) >> 5;
+  const int groups = ((N + 127) >> 7) * 32;
+  for (int g = warp; g < groups; g += nwarps) {
+    const int n0 = (g >> 5) * 128 + (g & 31);
+    float acc[4][TM];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int m = 0; m < TM; ++m) acc[j][m] = 0.f;
+    for (int c = lane; c < pieces; c += 32) {
+      const uint4 sw = __ldg(reinterpret_cast<const uint4*>(w_scales + fp4_scale_word(n0, NV ? c : c >> 1, tiles)));
+      const uint32_t sword[4] = {sw.x, sw.y, sw.z, sw.w};
+      uint4 wv[4][2];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int n = n0 + 32 * j;
+        const uint4* wrow = reinterpret_cast<const uint4*>(w_codes + (int64_t)n * (K >> 1));
+        wv[j][0] = n < N ? __ldcs(wrow + 2 * c) : make_uint4(0, 0, 0, 0);
+        wv[j][1] = n < N && 2 * c + 1 < chunks ? __ldcs(wrow + 2 * c + 1) : make_uint4(0, 0, 0, 0);
+      }
+      float as[TM][4];
+#pragma unroll
+      for (int m = 0; m < TM; ++m) {
+        const float4 t = s_s[m * pieces + c];
+        as[m][0] = t.x; as[m][1] = t.y; as[m][2] = t.z; as[m][3] = t.w;
+      }
+      float ws[4][4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) piece_scales<NV>(sword[j], c, ws[j]);
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {  // blocks of 16: two 16-byte reads of activations, 8 bytes of each column's codes
+        uint4 av[TM][2];
+#pragma unroll
+        for (int m = 0; m < TM; ++m) {
+          av[m][0] = s_a[(m * 8 + 2 * b) * pieces + c];
+          av[m][1] = s_a[(m * 8 + 2 * b + 1) * pieces + c];
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint4 q = wv[j][b >> 1];
+          uint32_t f0[4], f1[4];
+          e2m1x8_to_half2((b & 1) ? q.z : q.x, f0);
+          e2m1x8_to_half2((b & 1) ? q.w : q.y, f1);
+          auto h2 = [](const uint32_t& u) { return *reinterpret_cast<const __half2*>(&u); };
+#pragma unroll
+          for (int m = 0; m < TM; ++m) {
+            __half2 t = __hmul2(h2(f0[0]), h2(av[m][0].x));
+            t = __hfma2(h2(f0[1]), h2(av[m][0].y), t);
+            t = __hfma2(h2(f0[2]), h2(av[m][0].z), t);
+            t = __hfma2(h2(f0[3]), h2(av[m][0].w), t);
+            t = __hfma2(h2(f1[0]), h2(av[m][1].x), t);
+            t = __hfma2(h2(f1[1]), h2(av[m][1].y), t);
+            t = __hfma2(h2(f1[2]), h2(av[m][1].z), t);
+            t = __hfma2(h2(f1[3]), h2(av[m][1].w), t);
+            const float2 d = __half22float2(t);
+            acc[j][m] = fmaf(d.x + d.y, ws[j][b] * as[m][b], acc[j][m]);
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int m = 0; m < TM; ++m) acc[j][m] = warp_sum(acc[j][m]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {  // lane j writes column j
+      const int n = n0 + 32 * j;
+      if (lane == j && n < N) {
+        const float cs = rw != nullptr ? __ldg(rw + n) : 1.f;
+        const float b = bias != nullptr ? (float)bias[n] : 0.f;
+#pragma unroll
+        for (int m = 0; m < TM; ++m) {
+          float v = fmaf(acc[j][m] * (ra != nullptr ? __ldg(ra + m) : 1.f), cs, b);
+          if (gelu) v = gelu_tanh(v);
+          out[(int64_t)m * ld_out + n] = (T)v;
+        }
+      }
+    }
+  }
+}
+
+// ---- host side -----------------------------------------------------------------------------------------------
+static bool f4_map(CUtensorMap* map, CUtensorMapDataType type, int rank, const void* base, const cuuint64_t* dims,
+                   const cuuint64_t* strides, const cuuint32_t* box, bool swizzle) {
+  const EncodeTiledFn fn = tensor_map_encoder();
+  const cuuint32_t ones[3] = {1, 1, 1};
+  return fn != nullptr &&
+         fn(map, type, (cuuint32_t)rank, const_cast<void*>(base), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+static bool f4_code_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int box_rows) {
+  const cuuint64_t dims[2] = {(cuuint64_t)cols / 2, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)cols / 2};
+  const cuuint32_t box[2] = {128, (cuuint32_t)box_rows};
+  return f4_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, base, dims, strides, box, true);
+}
+// Scales as [panels, 4 * tiles, 128 bytes]; one step is a box of 4 * TILES lines of `panels` panels.
+static bool f4_scale_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, bool nv, int panels) {
+  const cuuint64_t lines = (cuuint64_t)fp4_panel_tiles(cols, nv) * 4;
+  const cuuint64_t dims[3] = {128, lines, (cuuint64_t)(rows + 127) / 128}, strides[2] = {128, lines * 128};
+  const cuuint32_t box[3] = {128, nv ? 16u : 8u, (cuuint32_t)panels};
+  return f4_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, base, dims, strides, box, false);
+}
+
+struct F4Plan {
+  bool pair;
+  int bn;
+};
+// Tile shape of a launch: the fewest waves of the cheapest tiles.  A step of a 256-column pair tile is the unit; costs
+// are relative clocks per step of 256 columns of K.
+static F4Plan f4_plan(int64_t M, int64_t N, int sms) {
+  const struct { bool pair; int bn; double step; } shapes[] = {{true, 256, 1.0}, {true, 128, 0.7}, {false, 128, 0.7}, {false, 64, 0.5}};
+  F4Plan best{true, 256};
+  double best_cost = 1e300;
+  for (const auto& s : shapes) {
+    if (s.pair && M <= 128) continue;
+    const int64_t bm = s.pair ? 256 : 128;
+    const int64_t tiles = ((M + bm - 1) / bm) * ((N + s.bn - 1) / s.bn);
+    const int64_t slots = s.pair ? sms / 2 : sms;
+    const double cost = (double)((tiles + slots - 1) / slots) * s.step;
+    if (cost < best_cost) {
+      best_cost = cost;
+      best = F4Plan{s.pair, s.bn};
+    }
+  }
+  return best;
+}
+
+template <int CG, bool NV, typename T>
+static int f4_launch(F4Params& p, int32_t* status_word, cudaStream_t st) {
+  static PerDevice attr_state;
+  const cudaError_t attr_err = (cudaError_t)attr_state.get([]() -> int64_t {
+    return (int64_t)cudaFuncSetAttribute(fp4_gemm_kernel<CG, NV, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, F4_SMEM_LIMIT);
+  });
+  CDB_CUDA_CHECK(attr_err);
+  const int slots = CG == 2 ? sm_count() / 2 : sm_count();
+  const unsigned grid = (unsigned)((p.num_tiles < slots ? p.num_tiles : slots) * CG);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(F4_THREADS);
+  cfg.dynamicSmemBytes = (size_t)(F4_FIXED_BYTES + p.stages * p.stage_bytes);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = CG;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = CG == 2 ? 1 : 0;
+  CDB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, fp4_gemm_kernel<CG, NV, T>, p, status_word));
+  return CDB_OK;
+}
+
+struct F4Matrix {  // mirrors `cdb_fp4_matrix` of the public header
+  const void* codes;
+  const void* block_scales;
+  const float* row_scale;
+};
+
+template <bool NV, typename T>
+static int f4_gemv(const F4Matrix& a, const F4Matrix& w, const void* bias, void* out, int64_t M, int64_t N, int64_t K,
+                   int64_t ld_out, int gelu, cudaStream_t st) {
+  const size_t smem = (size_t)M * f4v_row_bytes((int)((K + 63) / 64));
+  const int64_t want = ((N + 127) / 128 * 32 + F4V_THREADS / 32 - 1) / (F4V_THREADS / 32);
+#define CDB_F4V(TM)                                                                                                      \
+  do {                                                                                                                   \
+    static PerDevice resident;                                                                                           \
+    const int64_t per_sm = resident.get([]() -> int64_t {                                                                \
+      return -(int64_t)cudaFuncSetAttribute(fp4_gemv_kernel<TM, NV, T>, cudaFuncAttributeMaxDynamicSharedMemorySize,     \
+                                            F4V_SMEM_LIMIT);                                                             \
+    });                                                                                                                  \
+    CDB_CUDA_CHECK((cudaError_t)(-per_sm));                                                                              \
+    const int64_t cap = (int64_t)sm_count() * 4;                                                                         \
+    CDB_CUDA_CHECK(launch_pdl(fp4_gemv_kernel<TM, NV, T>, dim3((unsigned)(want < cap ? want : cap)), dim3(F4V_THREADS), \
+                              smem, st, static_cast<const uint8_t*>(a.codes), static_cast<const uint8_t*>(a.block_scales), \
+                              a.row_scale, static_cast<const uint8_t*>(w.codes),                                         \
+                              static_cast<const uint8_t*>(w.block_scales), w.row_scale, static_cast<const T*>(bias),     \
+                              static_cast<T*>(out), ld_out, (int)N, (int)K, gelu));                                      \
+  } while (0)
+  if (M == 1) CDB_F4V(1);
+  else if (M == 2) CDB_F4V(2);
+  else if (M == 3) CDB_F4V(3);
+  else CDB_F4V(4);
+#undef CDB_F4V
+  return CDB_OK;
+}
+
+template <bool NV, typename T>
+static int f4_gemm(const F4Matrix& a, const F4Matrix& w, const void* bias, void* out, int64_t M, int64_t N, int64_t K,
+                   int64_t ld_out, int gelu, int32_t* status_word, cudaStream_t st) {
+  if (M <= F4V_MAX_M && M * f4v_row_bytes((int)((K + 63) / 64)) <= F4V_SMEM_LIMIT)
+    return f4_gemv<NV, T>(a, w, bias, out, M, N, K, ld_out, gelu, st);
+  const F4Plan plan = f4_plan(M, N, sm_count());
+  const int cg = plan.pair ? 2 : 1, bn = plan.bn;
+  const int panels = bn > 128 ? bn / 128 : 1;
+  F4Params p{};
+  const cuuint64_t odims[2] = {(cuuint64_t)N, (cuuint64_t)M}, ostrides[1] = {(cuuint64_t)ld_out * 2};
+  const cuuint32_t obox[2] = {64, 32};
+  if (!f4_code_map(&p.map_a, a.codes, M, K, 128) || !f4_code_map(&p.map_w, w.codes, N, K, bn / cg) ||
+      !f4_scale_map(&p.map_sa, a.block_scales, M, K, NV, 1) || !f4_scale_map(&p.map_sw, w.block_scales, N, K, NV, panels) ||
+      !f4_map(&p.map_out, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, out, odims, ostrides, obox, true)) {
+    set_cuda_error(cudaErrorUnknown, "cuTensorMapEncodeTiled");
+    return CDB_ERR_CUDA;
+  }
+  p.ra = NV ? a.row_scale : nullptr;
+  p.rw = NV ? w.row_scale : nullptr;
+  p.bias = bias;
+  p.M = (int)M;
+  p.N = (int)N;
+  p.m_tiles = (int)((M + 128 * cg - 1) / (128 * cg));
+  p.n_tiles = (int)((N + bn - 1) / bn);
+  p.k_steps = (int)((K + FP4_STEP_COLS - 1) / FP4_STEP_COLS);
+  const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles;
+  if (tiles > INT32_MAX) return CDB_ERR_TOO_LARGE;
+  p.num_tiles = (int)tiles;
+  const int groups = (p.m_tiles + 15) / 16;
+  p.group_m = p.m_tiles <= 24 ? p.m_tiles : (p.m_tiles + groups - 1) / groups;
+  p.bn = bn;
+  p.gelu = gelu != 0;
+  p.idesc = f4_idesc(128 * cg, bn, NV);
+  p.stage_bytes = F4_A_BYTES + bn / cg * 128 + (NV ? 4 : 2) * 512 * (1 + panels);
+  const int fit = (F4_SMEM_LIMIT - F4_FIXED_BYTES) / p.stage_bytes;
+  p.stages = fit < F4_MAX_STAGES ? fit : F4_MAX_STAGES;
+  return plan.pair ? f4_launch<2, NV, T>(p, status_word, st) : f4_launch<1, NV, T>(p, status_word, st);
+}
+
+}  // namespace cdb
+
+using namespace cdb;
+
+extern "C" int cdb_fp4_gemm(const void* a_v, const void* w_v, const void* bias, void* out, int64_t M, int64_t N, int64_t K,
+                            int64_t ld_out, int format, int dtype, int gelu, int32_t* status_word, void* stream) {
+  const F4Matrix* a = static_cast<const F4Matrix*>(a_v);
+  const F4Matrix* w = static_cast<const F4Matrix*>(w_v);
+  if (!a || !w || M < 0 || N <= 0 || K <= 0 || ld_out < N || (format != CDB_NVFP4 && format != CDB_MXFP4) ||
+      (dtype != CDB_BF16 && dtype != CDB_F16))
+    return CDB_ERR_BAD_ARGUMENT;
+  if (M == 0) return CDB_OK;
+  const bool nv = format == CDB_NVFP4;
+  if (!a->codes || !a->block_scales || !w->codes || !w->block_scales || !out || (nv && (!a->row_scale || !w->row_scale)))
+    return CDB_ERR_BAD_ARGUMENT;
+  if (K % 32 != 0 || K > FP4_MAX_COLS || N % 8 != 0 || ld_out % 8 != 0 || M > INT32_MAX || N > INT32_MAX ||
+      !aligned16(a->codes) || !aligned16(a->block_scales) || !aligned16(w->codes) || !aligned16(w->block_scales) ||
+      !aligned16(out))
+    return CDB_ERR_UNSUPPORTED;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (dtype == CDB_BF16)
+    return nv ? f4_gemm<true, __nv_bfloat16>(*a, *w, bias, out, M, N, K, ld_out, gelu, status_word, st)
+              : f4_gemm<false, __nv_bfloat16>(*a, *w, bias, out, M, N, K, ld_out, gelu, status_word, st);
+  return nv ? f4_gemm<true, __half>(*a, *w, bias, out, M, N, K, ld_out, gelu, status_word, st)
+            : f4_gemm<false, __half>(*a, *w, bias, out, M, N, K, ld_out, gelu, status_word, st);
+}

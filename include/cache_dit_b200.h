@@ -29,6 +29,9 @@ extern "C" {
 /* Storage dtype of activation tensors. */
 enum cdb_dtype { CDB_F32 = 0, CDB_BF16 = 1, CDB_F16 = 2 };
 
+/* 4-bit microscaled formats (see cdb_fp4_quant_rows). */
+enum cdb_fp4_format { CDB_NVFP4 = 0, CDB_MXFP4 = 1 };
+
 /* Status codes. */
 enum cdb_status {
   CDB_OK = 0,
@@ -349,6 +352,42 @@ CDB_API int cdb_gated_residual_pair(const void* x, const void* y, int64_t ld_y, 
                             void* out, int64_t rows, int64_t rows_per_batch, const void* x2, const void* y2,
                             int64_t ld_y2, const void* gate2, int64_t ld_gate2, void* out2, int64_t rows2,
                             int64_t rows_per_batch2, int64_t cols, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * 4-bit microscaled matrices.  Beside the reference's `nvfp4` quantization type
+ * (src/cache_dit/quantization/torchao/quantize_ao.py), with a second-level scale per row instead of per tensor.
+ *
+ *   CDB_NVFP4  blocks of 16 columns: x ~ code * scale * row_scale[r]; scale e4m3, row_scale the smallest power of two
+ *              >= max(max|x_r| / 2688, 2^-100); scale = e4m3(max|block| / (6 row_scale))
+ *   CDB_MXFP4  blocks of 32 columns: x ~ code * scale; scale = 2^(floor(log2(max|block|)) - 2), e8m0, at least 2^-127
+ * A code is the e2m1 number (0 0.5 1 1.5 2 3 4 6) nearest to x / (scale * row_scale), ties to the even code,
+ * saturating.  codes [rows, cols/2], contiguous, the even column in the low four bits.  block_scales has
+ * cdb_fp4_block_scale_bytes(): tiles of 128 rows x 4 scales = 512 bytes, byte (r%32)*16 + (r%128/32)*4 + k%4; the tiles
+ * of a panel of 128 rows lie one after another, padded with zeros to whole steps of 256 columns.  row_scale [rows]
+ * float32 for CDB_NVFP4, NULL (not read) for CDB_MXFP4.
+ * An infinity or NaN makes its row (CDB_NVFP4) or block (CDB_MXFP4) stand for NaN.
+ * x: `dtype` rows, ld_x elements apart.  cols % 32 == 0, cols <= 16384, pointers and rows 16-byte aligned.
+ * cdb_fp4_dequant_rows writes the values (fp32 products, rounded once) as contiguous `dtype` rows.
+ * ---------------------------------------------------------------------------------------- */
+CDB_API size_t cdb_fp4_block_scale_bytes(int64_t rows, int64_t cols, int format);
+CDB_API int cdb_fp4_quant_rows(const void* x, int64_t rows, int64_t cols, int64_t ld_x, int dtype, int format,
+                               void* codes, void* block_scales, float* row_scale, void* stream);
+CDB_API int cdb_fp4_dequant_rows(const void* codes, const void* block_scales, const float* row_scale, int64_t rows,
+                                 int64_t cols, int format, void* out, int dtype, void* stream);
+
+/* out[m, n] = act(sum_k a[m, k] w[n, k] + bias[n]) for two 4-bit matrices of one format, a [M, K] and w [N, K].
+ * fp32 accumulation in tensor memory (tcgen05, block scales applied by the tensor core); out [M, N] and bias [N]
+ * (or NULL) are `dtype` (CDB_BF16 or CDB_F16), out rows ld_out elements apart; gelu != 0: act is the tanh-GELU of the
+ * fp32 value, else the identity; rounded once.  K % 32 == 0, K <= 16384, N % 8 == 0, pointers and rows 16-byte aligned.
+ * `status_word` as in cdb_fp8_gemm_rowscaled. */
+typedef struct cdb_fp4_matrix {
+  const void* codes;
+  const void* block_scales;
+  const float* row_scale; /* NULL for CDB_MXFP4 */
+} cdb_fp4_matrix;
+CDB_API int cdb_fp4_gemm(const void* a /* cdb_fp4_matrix */, const void* w /* cdb_fp4_matrix */, const void* bias,
+                         void* out, int64_t M, int64_t N, int64_t K, int64_t ld_out, int format, int dtype, int gelu,
+                         int32_t* status_word, void* stream);
 
 #ifdef __cplusplus
 }
