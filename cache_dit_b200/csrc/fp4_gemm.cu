@@ -18,6 +18,7 @@
 // Every wait is bounded (bounded_wait): on expiry the roles drain, tensor memory is freed and the kernel returns.
 #include <cuda_fp16.h>
 
+#include <atomic>
 #include <cstdlib>
 
 #include "fp4.cuh"
@@ -33,8 +34,6 @@ constexpr int F4_MAX_BN = 256;
 constexpr int F4_A_BYTES = 128 * 128;     // 128 rows of one step's codes
 constexpr uint32_t F4_TMEM_COLS = 512;
 constexpr uint32_t F4_SHARED_COL = 160;   // where the second accumulator starts when bn = 256
-constexpr uint32_t F4_SF_COL = 416;       // scales: two slots of 48 columns (16 for A, 32 for W)
-constexpr uint32_t F4_SF_SLOT = 48;
 constexpr int F4_BLOCK_BYTES = 32 * 64 * 2;                      // one staged block of output: 32 rows x 64 columns
 constexpr int F4_STAGING_BYTES = (F4_EPI_THREADS / 32) * 2 * F4_BLOCK_BYTES;
 constexpr int F4_SMEM_LIMIT = 232448;
@@ -56,7 +55,8 @@ struct F4Params {
   const void* bias;
   int M, N;
   int m_tiles, n_tiles, k_steps, group_m, num_tiles;
-  int bn, stages, stage_bytes, gelu;
+  int stages, stage_bytes, gelu;
+  uint32_t sf_col, slots;
   uint32_t idesc;
 };
 
@@ -73,20 +73,29 @@ __device__ __forceinline__ void tma_load_3d_pair(const CUtensorMap* map, uint32_
       ::"r"(smem_u32(dst)), "l"(map), "r"(bar_cluster_addr), "r"(c0), "r"(c1), "r"(c2)
       : "memory");
 }
+// tcgen05 instructions of a whole, converged warp: each elects its issuing lane itself.  Under a branch on an elected
+// lane every operand had to be made uniform by hand of the compiler, about 60 clocks an instruction.
+#define CDB_ELECTED(text) "{\n\t.reg .pred e, p;\n\telect.sync _|e, 0xffffffff;\n\t" text "\n\t}"
 // 32 rows x 16 bytes of shared memory -> 4 tensor memory columns, the same in all four lane quarters (CG = 2: in both
 // CTAs, each from its own shared memory).
 template <int CG>
 __device__ __forceinline__ void copy_scales(uint32_t tmem, uint64_t desc) {
-  if constexpr (CG == 2) asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
-  else asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+  if constexpr (CG == 2) asm volatile(CDB_ELECTED("@e tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;") ::"r"(tmem), "l"(desc) : "memory");
+  else asm volatile(CDB_ELECTED("@e tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;") ::"r"(tmem), "l"(desc) : "memory");
 }
-#define CDB_F4_MMA(CG_, KIND_)                                                                                  \
-  asm volatile(                                                                                                 \
-      "{\n\t.reg .pred p;\n\t"                                                                                  \
-      "setp.ne.b32 p, %6, 0;\n\t"                                                                               \
-      "tcgen05.mma.cta_group::" CG_ ".kind::" KIND_ " [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(tmem_d),      \
-      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)                                    \
-      : "memory")
+template <int CG>
+__device__ __forceinline__ void commit_warp(uint32_t bar) {
+  if constexpr (CG == 2)
+    asm volatile(CDB_ELECTED("@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;")
+                 ::"r"(bar), "h"((uint16_t)3) : "memory");
+  else
+    asm volatile(CDB_ELECTED("@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];") ::"r"(bar) : "memory");
+}
+#define CDB_F4_MMA(CG_, KIND_)                                                                                      \
+  asm volatile(CDB_ELECTED("setp.ne.b32 p, %6, 0;\n\t"                                                              \
+                           "@e tcgen05.mma.cta_group::" CG_ ".kind::" KIND_ " [%0], %1, %2, %3, [%4], [%5], p;")     \
+               ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)                \
+               : "memory")
 template <int CG, bool NV>
 __device__ __forceinline__ void mma_f4(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t sfa,
                                        uint32_t sfb, uint32_t accumulate) {
@@ -105,6 +114,18 @@ constexpr uint32_t f4_idesc(int m, int n, bool nv) {
 __device__ __forceinline__ uint64_t scale_tile_desc(uint32_t smem_addr) {
   return (uint64_t)((smem_addr & 0x3FFFFu) >> 4) | ((uint64_t)(128 >> 4) << 16) | ((uint64_t)(128 >> 4) << 32) | ((uint64_t)1 << 46);
 }
+// Position in the ring of stages: index and phase bit, advanced without the divisions that would sit in every step's
+// serial chain (they took more clocks than a step's MMAs).
+struct RingPos {
+  int stage = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void next(int stages) {
+    if (++stage == stages) {
+      stage = 0;
+      phase ^= 1u;
+    }
+  }
+};
 // M fastest inside groups of `group_m` row tiles, so a wave shares weight tiles and a bounded set of A panels in L2.
 __device__ __forceinline__ void f4_tile_coords(int tile, const F4Params& p, int& mi, int& ni) {
   const int per_group = p.group_m * p.n_tiles;
@@ -174,7 +195,7 @@ __device__ __forceinline__ void f4_store_block(const F4Params& p, uint8_t* stagi
   ++blocks_done;
 }
 
-template <int CG, bool NV, typename T>
+template <int CG, int BN, bool NV, typename T>
 __global__ void __launch_bounds__(F4_THREADS, 1) fp4_gemm_kernel(const __grid_constant__ F4Params p, int32_t* status_word) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -183,18 +204,17 @@ __global__ void __launch_bounds__(F4_THREADS, 1) fp4_gemm_kernel(const __grid_co
   F4Barriers* gb = reinterpret_cast<F4Barriers*>(s_col + F4_MAX_BN);
 
   constexpr int TILES = NV ? 4 : 2;  // scale tiles of one step and panel
-  const int warp = threadIdx.x >> 5;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);  // uniform to the compiler as well
   const int lane = threadIdx.x & 31;
   const uint32_t rank = CG == 2 ? cluster_ctarank() : 0u;  // 0 owns the shared barriers and issues the MMAs
   const int first = CG == 2 ? blockIdx.x >> 1 : blockIdx.x;
   const int step = CG == 2 ? gridDim.x >> 1 : gridDim.x;
-  const int bn = p.bn;
-  const int panels = bn > 128 ? bn / 128 : 1;
-  const uint32_t b_bytes = (uint32_t)(CG == 2 ? bn >> 1 : bn) * 128u;
-  const uint32_t sfa_off = F4_A_BYTES + b_bytes;
-  const uint32_t sfb_off = sfa_off + TILES * 512;
-  const bool shared_acc = bn == F4_MAX_BN;
-  const uint32_t acc1 = shared_acc ? F4_SHARED_COL : (uint32_t)bn;
+  constexpr int bn = BN;
+  constexpr int PANELS = BN > 128 ? BN / 128 : 1;  // of 128 weight rows: one tile's scales
+  constexpr uint32_t sfa_off = F4_A_BYTES + BN / CG * 128;
+  constexpr uint32_t sfb_off = sfa_off + TILES * 512;
+  constexpr bool shared_acc = BN == F4_MAX_BN;
+  constexpr uint32_t acc1 = shared_acc ? F4_SHARED_COL : BN;
   const int stages = p.stages;
   pdl_launch_dependents();
 
@@ -223,23 +243,24 @@ __global__ void __launch_bounds__(F4_THREADS, 1) fp4_gemm_kernel(const __grid_co
   __syncthreads();
   if constexpr (CG == 2) cluster_sync_all();  // the peer's barriers exist before anything is signalled across the pair
   tcgen05_fence_after();
-  const uint32_t tmem_base = gb->tmem_base;
+  const uint32_t tmem_base = __shfl_sync(0xffffffffu, gb->tmem_base, 0);
 
   if (warp == 0) {
     // ---------------- TMA producer ----------------
     if (lane == 0) {
-      uint32_t it = 0;
+      RingPos at;
+      uint32_t issued = 0;
       bool ok = true;
-      const uint32_t tx = CG * (sfb_off + (uint32_t)panels * TILES * 512);  // both CTAs' bytes of one stage
+      constexpr uint32_t tx = CG * (sfb_off + PANELS * TILES * 512);  // both CTAs' bytes of one stage
       for (int tile = first; tile < p.num_tiles && ok; tile += step) {
         int mi, ni;
         f4_tile_coords(tile, p, mi, ni);
         const int m0 = mi * (128 * CG) + (int)rank * 128;
         const int n0 = ni * bn;
         const int w0 = n0 + (CG == 2 ? (int)rank * (bn >> 1) : 0);
-        for (int kb = 0; kb < p.k_steps; ++kb, ++it) {
-          const int s = it % stages;
-          ok = bounded_wait(&gb->empty[s], ((it / stages) & 1u) ^ 1u, &gb->abort_flag, status_word, 21);
+        for (int kb = 0; kb < p.k_steps; ++kb, at.next(stages), ++issued) {
+          const int s = at.stage;
+          ok = bounded_wait(&gb->empty[s], at.phase ^ 1u, &gb->abort_flag, status_word, 21);
           if (!ok) break;
           uint8_t* dst = smem + s * p.stage_bytes;
           if constexpr (CG == 2) {
@@ -261,7 +282,7 @@ __global__ void __launch_bounds__(F4_THREADS, 1) fp4_gemm_kernel(const __grid_co
       // A CTA may not retire while copies into its shared memory are in flight or while MMAs read it: wait (bounded,
       // also after an abort) until the MMAs released every stage used.
       const uint64_t t0 = global_timer_ns();
-      for (uint32_t j = (it > (uint32_t)stages ? it - stages : 0); j < it; ++j) {
+      for (uint32_t j = (issued > (uint32_t)stages ? issued - stages : 0); j < issued; ++j) {
         while (!mbar_try_wait(&gb->empty[j % stages], (j / stages) & 1u)) {
           if (global_timer_ns() - t0 > BARRIER_LIMIT_NS) break;
         }
@@ -270,17 +291,20 @@ __global__ void __launch_bounds__(F4_THREADS, 1) fp4_gemm_kernel(const __grid_co
     __syncwarp();
   } else if (warp == 1) {
     // ---------------- MMA issuer ----------------
-    if (lane == 0 && rank == 0) {
-      uint32_t it = 0, n_tile = 0;
-      bool ok = true;
+    if (rank == 0) {  // the whole warp waits, one elected lane issues
+      const uint32_t slots = p.slots, slot_cols = TILES * 4 * (1 + PANELS);
+      const uint32_t smem_base = __shfl_sync(0xffffffffu, smem_u32(smem), 0);
+      RingPos at, old;  // `old`: the step whose scale slot is written next
+      uint32_t slot = 0, n_tile = 0;
+      bool ok = true, slots_used = false;
       for (int tile = first; tile < p.num_tiles && ok; tile += step, ++n_tile) {
         const uint32_t buf = n_tile & 1u;
         // Separate accumulators: tile n_tile - 2 has left this one.  Shared columns: tile n_tile - 1 has left them
         // (and n_tile - 2 everything, since the epilogue takes tiles in order).
         if (!shared_acc) {
-          ok = bounded_wait(&gb->acc_empty[buf], ((n_tile >> 1) & 1u) ^ 1u, &gb->abort_flag, status_word, 22);
+          ok = __all_sync(0xffffffffu, bounded_wait(&gb->acc_empty[buf], ((n_tile >> 1) & 1u) ^ 1u, &gb->abort_flag, status_word, 22));
         } else if (n_tile > 0) {
-          ok = bounded_wait(&gb->acc_empty[buf ^ 1u], ((n_tile - 1) >> 1) & 1u, &gb->abort_flag, status_word, 22);
+          ok = __all_sync(0xffffffffu, bounded_wait(&gb->acc_empty[buf ^ 1u], ((n_tile - 1) >> 1) & 1u, &gb->abort_flag, status_word, 22));
         }
         if (!ok) break;
         tcgen05_fence_after();
@@ -289,26 +313,27 @@ __global__ void __launch_bounds__(F4_THREADS, 1) fp4_gemm_kernel(const __grid_co
         f4_tile_coords(tile, p, mi, ni);
         // a 64-column tile may be the second half of its panel of 128 weight rows: scales two columns on
         const uint32_t sfb_skip = (uint32_t)((ni * bn) & 127) >> 5;
-        for (int kb = 0; kb < p.k_steps; ++kb, ++it) {
-          const int s = it % stages;
-          ok = bounded_wait(&gb->full[s], (it / stages) & 1u, &gb->abort_flag, status_word, 23);
+        for (int kb = 0; kb < p.k_steps; ++kb, at.next(stages)) {
+          const int s = at.stage;
+          ok = __all_sync(0xffffffffu, bounded_wait(&gb->full[s], at.phase, &gb->abort_flag, status_word, 23));
           if (!ok) break;
-          // The scale slot of this step was read by the MMAs of step it - 2: they have retired when their stage is
-          // released.  The MMAs of step it - 1 are still queued, so the tensor pipe does not run dry meanwhile.
-          if (it >= 2) {
-            const uint32_t u = it - 2;
-            ok = bounded_wait(&gb->empty[u % stages], (u / stages) & 1u, &gb->abort_flag, status_word, 24);
+          // The slot's last readers are the MMAs of `slots` steps ago: they have retired when their stage is released.
+          // The MMAs of the steps between are still queued, so the tensor pipe does not run dry meanwhile.
+          if (slots_used) {
+            ok = __all_sync(0xffffffffu, bounded_wait(&gb->empty[old.stage], old.phase, &gb->abort_flag, status_word, 24));
             if (!ok) break;
+            old.next(stages);
           }
           tcgen05_fence_after();
-          const uint32_t base = smem_u32(smem + s * p.stage_bytes);
-          const uint32_t sfa = tmem_base + F4_SF_COL + (it & 1u) * F4_SF_SLOT;
-          const uint32_t sfb = sfa + 16;
+          const uint32_t base = smem_base + (uint32_t)s * (uint32_t)p.stage_bytes;
+          const uint32_t sfa = tmem_base + p.sf_col + slot * slot_cols;
+          const uint32_t sfb = sfa + TILES * 4;
 #pragma unroll
           for (int j = 0; j < TILES; ++j) {
             copy_scales<CG>(sfa + j * 4, scale_tile_desc(base + sfa_off + j * 512));
-            for (int q = 0; q < panels; ++q)
-              copy_scales<CG>(sfb + (j * panels + q) * 4, scale_tile_desc(base + sfb_off + (q * TILES + j) * 512));
+#pragma unroll
+            for (int q = 0; q < PANELS; ++q)
+              copy_scales<CG>(sfb + (j * PANELS + q) * 4, scale_tile_desc(base + sfb_off + (q * TILES + j) * 512));
           }
           const uint64_t adesc = make_kmajor_sw128_desc(base);
           const uint64_t bdesc = make_kmajor_sw128_desc(base + F4_A_BYTES);
@@ -317,15 +342,15 @@ __global__ void __launch_bounds__(F4_THREADS, 1) fp4_gemm_kernel(const __grid_co
             const int j = NV ? k : k >> 1;
             const uint32_t id = NV ? 0u : (uint32_t)(k & 1) * 2u;
             mma_f4<CG, NV>(tmem_d, adesc + 2 * k, bdesc + 2 * k, p.idesc | (id << 4) | (id << 29), sfa + j * 4,
-                           sfb + j * panels * 4 + sfb_skip, (kb | k) != 0 ? 1u : 0u);
+                           sfb + j * PANELS * 4 + sfb_skip, (kb | k) != 0 ? 1u : 0u);
           }
-          if constexpr (CG == 2) tcgen05_commit_both(smem_u32(&gb->empty[s]));
-          else tcgen05_commit(&gb->empty[s]);
+          commit_warp<CG>(smem_u32(&gb->empty[s]));
+          if (++slot == slots) {
+            slot = 0;
+            slots_used = true;
+          }
         }
-        if (ok) {
-          if constexpr (CG == 2) tcgen05_commit_both(smem_u32(&gb->acc_full[buf]));
-          else tcgen05_commit(&gb->acc_full[buf]);
-        }
+        if (ok) commit_warp<CG>(smem_u32(&gb->acc_full[buf]));
       }
     }
     __syncwarp();
@@ -379,7 +404,7 @@ __global__ void __launch_bounds__(F4_THREADS, 1) fp4_gemm_kernel(const __grid_co
           f4_store_block<T>(p, staging, blocks_done, lo, hi, c, n0, row0, rs, s_col, lane);
         }
       };
-      if (!shared_acc) {
+      if constexpr (!shared_acc) {
         if (live) plain_blocks(0, bn);
         release();
       } else if (!live) {
@@ -588,10 +613,14 @@ struct F4Plan {
   bool pair;
   int bn;
 };
+// Tuning / testing knob: 0 = chosen by size, else the tile's columns, negative for a CTA pair's.
+static std::atomic<int> g_f4_tile{0};
 // Tile shape of a launch: the fewest waves of the cheapest tiles.  A step of a 256-column pair tile is the unit; costs
 // are relative clocks per step of 256 columns of K.
 static F4Plan f4_plan(int64_t M, int64_t N, int sms) {
   const struct { bool pair; int bn; double step; } shapes[] = {{true, 256, 1.0}, {true, 128, 0.7}, {false, 128, 0.7}, {false, 64, 0.5}};
+  const int forced = g_f4_tile.load(std::memory_order_relaxed);
+  if (forced != 0) return F4Plan{forced < 0, forced < 0 ? -forced : forced};
   F4Plan best{true, 256};
   double best_cost = 1e300;
   for (const auto& s : shapes) {
@@ -608,11 +637,11 @@ static F4Plan f4_plan(int64_t M, int64_t N, int sms) {
   return best;
 }
 
-template <int CG, bool NV, typename T>
+template <int CG, int BN, bool NV, typename T>
 static int f4_launch(F4Params& p, int32_t* status_word, cudaStream_t st) {
   static PerDevice attr_state;
   const cudaError_t attr_err = (cudaError_t)attr_state.get([]() -> int64_t {
-    return (int64_t)cudaFuncSetAttribute(fp4_gemm_kernel<CG, NV, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, F4_SMEM_LIMIT);
+    return (int64_t)cudaFuncSetAttribute(fp4_gemm_kernel<CG, BN, NV, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, F4_SMEM_LIMIT);
   });
   CDB_CUDA_CHECK(attr_err);
   const int slots = CG == 2 ? sm_count() / 2 : sm_count();
@@ -628,7 +657,7 @@ static int f4_launch(F4Params& p, int32_t* status_word, cudaStream_t st) {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = CG == 2 ? 1 : 0;
-  CDB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, fp4_gemm_kernel<CG, NV, T>, p, status_word));
+  CDB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, fp4_gemm_kernel<CG, BN, NV, T>, p, status_word));
   return CDB_OK;
 }
 
@@ -669,7 +698,7 @@ static int f4_gemv(const F4Matrix& a, const F4Matrix& w, const void* bias, void*
 template <bool NV, typename T>
 static int f4_gemm(const F4Matrix& a, const F4Matrix& w, const void* bias, void* out, int64_t M, int64_t N, int64_t K,
                    int64_t ld_out, int gelu, int32_t* status_word, cudaStream_t st) {
-  if (M <= F4V_MAX_M && M * f4v_row_bytes((int)((K + 63) / 64)) <= F4V_SMEM_LIMIT)
+  if (g_f4_tile.load(std::memory_order_relaxed) == 0 && M <= F4V_MAX_M && M * f4v_row_bytes((int)((K + 63) / 64)) <= F4V_SMEM_LIMIT)
     return f4_gemv<NV, T>(a, w, bias, out, M, N, K, ld_out, gelu, st);
   const F4Plan plan = f4_plan(M, N, sm_count());
   const int cg = plan.pair ? 2 : 1, bn = plan.bn;
@@ -696,18 +725,29 @@ static int f4_gemm(const F4Matrix& a, const F4Matrix& w, const void* bias, void*
   p.num_tiles = (int)tiles;
   const int groups = (p.m_tiles + 15) / 16;
   p.group_m = p.m_tiles <= 24 ? p.m_tiles : (p.m_tiles + groups - 1) / groups;
-  p.bn = bn;
   p.gelu = gelu != 0;
   p.idesc = f4_idesc(128 * cg, bn, NV);
   p.stage_bytes = F4_A_BYTES + bn / cg * 128 + (NV ? 4 : 2) * 512 * (1 + panels);
   const int fit = (F4_SMEM_LIMIT - F4_FIXED_BYTES) / p.stage_bytes;
   p.stages = fit < F4_MAX_STAGES ? fit : F4_MAX_STAGES;
-  return plan.pair ? f4_launch<2, NV, T>(p, status_word, st) : f4_launch<1, NV, T>(p, status_word, st);
+  // Scale slots: what the accumulators leave of tensor memory, and no more than stages.  The MMA issuer tells a slot's
+  // release by its stage's barrier, whose phase bit says nothing about a use more than one round of the ring ago.
+  p.sf_col = bn == F4_MAX_BN ? F4_SHARED_COL + F4_MAX_BN : 2 * bn;
+  const uint32_t fit_slots = (F4_TMEM_COLS - p.sf_col) / ((NV ? 16 : 8) * (1 + panels));
+  p.slots = fit_slots < (uint32_t)p.stages ? fit_slots : (uint32_t)p.stages;
+  if (plan.pair) return bn == 256 ? f4_launch<2, 256, NV, T>(p, status_word, st) : f4_launch<2, 128, NV, T>(p, status_word, st);
+  return bn == 128 ? f4_launch<1, 128, NV, T>(p, status_word, st) : f4_launch<1, 64, NV, T>(p, status_word, st);
 }
 
 }  // namespace cdb
 
 using namespace cdb;
+
+extern "C" int cdb_tuning_set_fp4_tile(int pair, int cols) {
+  if (cols != 0 && cols != 128 && cols != (pair ? 256 : 64)) return CDB_ERR_BAD_ARGUMENT;
+  g_f4_tile.store(pair ? -cols : cols, std::memory_order_relaxed);
+  return CDB_OK;
+}
 
 extern "C" int cdb_fp4_gemm(const void* a_v, const void* w_v, const void* bias, void* out, int64_t M, int64_t N, int64_t K,
                             int64_t ld_out, int format, int dtype, int gelu, int32_t* status_word, void* stream) {
