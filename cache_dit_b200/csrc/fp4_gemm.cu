@@ -14,7 +14,8 @@
 //     the next tile's MMAs wait for is that read.
 //   * M <= 4 rows: no tile; the weights are streamed once by the CUDA cores (fp4_gemv_kernel).
 //
-// Warp roles (192 threads): warp 0 = TMA producer, warp 1 = tensor memory owner and MMA issuer, warps 2..5 = epilogue.
+// Warp roles (224 threads): warp 0 = TMA producer, warp 1 = tensor memory owner and MMA issuer, warps 2..5 = epilogue,
+// warp 6 = block scales to tensor memory.
 // Every wait is bounded (bounded_wait): on expiry the roles drain, tensor memory is freed and the kernel returns.
 #include <cuda_fp16.h>
 
@@ -26,10 +27,12 @@
 
 namespace cdb {
 
-constexpr int F4_THREADS = 192;
+constexpr int F4_THREADS = 224;
 constexpr int F4_EPI_WARP0 = 2;
 constexpr int F4_EPI_THREADS = 128;
+constexpr int F4_SCALE_WARP = 6;
 constexpr int F4_MAX_STAGES = 8;
+constexpr int F4_MAX_SLOTS = 8;
 constexpr int F4_MAX_BN = 256;
 constexpr int F4_A_BYTES = 128 * 128;     // 128 rows of one step's codes
 constexpr uint32_t F4_TMEM_COLS = 512;
@@ -41,6 +44,7 @@ constexpr int F4_SMEM_LIMIT = 232448;
 struct __align__(8) F4Barriers {
   uint64_t full[F4_MAX_STAGES];
   uint64_t empty[F4_MAX_STAGES];
+  uint64_t sf_full[F4_MAX_SLOTS];  // block scales of a step are in tensor memory
   uint64_t acc_full[2];
   uint64_t acc_empty[2];
   uint32_t tmem_base;
@@ -56,7 +60,8 @@ struct F4Params {
   int M, N;
   int m_tiles, n_tiles, k_steps, group_m, num_tiles;
   int stages, stage_bytes, gelu;
-  uint32_t sf_col, slots;
+  uint32_t sf_col;
+  int slots;
   uint32_t idesc;
 };
 
@@ -88,6 +93,13 @@ __device__ __forceinline__ void commit_warp(uint32_t bar) {
   if constexpr (CG == 2)
     asm volatile(CDB_ELECTED("@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;")
                  ::"r"(bar), "h"((uint16_t)3) : "memory");
+  else
+    asm volatile(CDB_ELECTED("@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];") ::"r"(bar) : "memory");
+}
+template <int CG>
+__device__ __forceinline__ void commit_own(uint32_t bar) {  // to this CTA's barrier alone
+  if constexpr (CG == 2)
+    asm volatile(CDB_ELECTED("@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];") ::"r"(bar) : "memory");
   else
     asm volatile(CDB_ELECTED("@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];") ::"r"(bar) : "memory");
 }
@@ -213,6 +225,7 @@ __global__ void __launch_bounds__(F4_THREADS, 1) fp4_gemm_kernel(const __grid_co
   constexpr int PANELS = BN > 128 ? BN / 128 : 1;  // of 128 weight rows: one tile's scales
   constexpr uint32_t sfa_off = F4_A_BYTES + BN / CG * 128;
   constexpr uint32_t sfb_off = sfa_off + TILES * 512;
+  constexpr uint32_t SLOT_COLS = TILES * 4 * (1 + PANELS);
   constexpr bool shared_acc = BN == F4_MAX_BN;
   constexpr uint32_t acc1 = shared_acc ? F4_SHARED_COL : BN;
   const int stages = p.stages;
@@ -223,6 +236,7 @@ __global__ void __launch_bounds__(F4_THREADS, 1) fp4_gemm_kernel(const __grid_co
       mbar_init(&gb->full[s], 1);
       mbar_init(&gb->empty[s], 1);
     }
+    for (int i = 0; i < F4_MAX_SLOTS; ++i) mbar_init(&gb->sf_full[i], 1);
     for (int b = 0; b < 2; ++b) {
       mbar_init(&gb->acc_full[b], 1);
       mbar_init(&gb->acc_empty[b], CG * (F4_EPI_THREADS / 32));
@@ -292,11 +306,10 @@ __global__ void __launch_bounds__(F4_THREADS, 1) fp4_gemm_kernel(const __grid_co
   } else if (warp == 1) {
     // ---------------- MMA issuer ----------------
     if (rank == 0) {  // the whole warp waits, one elected lane issues
-      const uint32_t slots = p.slots, slot_cols = TILES * 4 * (1 + PANELS);
       const uint32_t smem_base = __shfl_sync(0xffffffffu, smem_u32(smem), 0);
-      RingPos at, old;  // `old`: the step whose scale slot is written next
-      uint32_t slot = 0, n_tile = 0;
-      bool ok = true, slots_used = false;
+      RingPos at, slot;
+      uint32_t n_tile = 0;
+      bool ok = true;
       for (int tile = first; tile < p.num_tiles && ok; tile += step, ++n_tile) {
         const uint32_t buf = n_tile & 1u;
         // Separate accumulators: tile n_tile - 2 has left this one.  Shared columns: tile n_tile - 1 has left them
@@ -317,24 +330,12 @@ __global__ void __launch_bounds__(F4_THREADS, 1) fp4_gemm_kernel(const __grid_co
           const int s = at.stage;
           ok = __all_sync(0xffffffffu, bounded_wait(&gb->full[s], at.phase, &gb->abort_flag, status_word, 23));
           if (!ok) break;
-          // The slot's last readers are the MMAs of `slots` steps ago: they have retired when their stage is released.
-          // The MMAs of the steps between are still queued, so the tensor pipe does not run dry meanwhile.
-          if (slots_used) {
-            ok = __all_sync(0xffffffffu, bounded_wait(&gb->empty[old.stage], old.phase, &gb->abort_flag, status_word, 24));
-            if (!ok) break;
-            old.next(stages);
-          }
+          ok = __all_sync(0xffffffffu, bounded_wait(&gb->sf_full[slot.stage], slot.phase, &gb->abort_flag, status_word, 24));
+          if (!ok) break;
           tcgen05_fence_after();
           const uint32_t base = smem_base + (uint32_t)s * (uint32_t)p.stage_bytes;
-          const uint32_t sfa = tmem_base + p.sf_col + slot * slot_cols;
+          const uint32_t sfa = tmem_base + p.sf_col + (uint32_t)slot.stage * SLOT_COLS;
           const uint32_t sfb = sfa + TILES * 4;
-#pragma unroll
-          for (int j = 0; j < TILES; ++j) {
-            copy_scales<CG>(sfa + j * 4, scale_tile_desc(base + sfa_off + j * 512));
-#pragma unroll
-            for (int q = 0; q < PANELS; ++q)
-              copy_scales<CG>(sfb + (j * PANELS + q) * 4, scale_tile_desc(base + sfb_off + (q * TILES + j) * 512));
-          }
           const uint64_t adesc = make_kmajor_sw128_desc(base);
           const uint64_t bdesc = make_kmajor_sw128_desc(base + F4_A_BYTES);
 #pragma unroll
@@ -345,12 +346,44 @@ __global__ void __launch_bounds__(F4_THREADS, 1) fp4_gemm_kernel(const __grid_co
                            sfb + j * PANELS * 4 + sfb_skip, (kb | k) != 0 ? 1u : 0u);
           }
           commit_warp<CG>(smem_u32(&gb->empty[s]));
-          if (++slot == slots) {
-            slot = 0;
-            slots_used = true;
-          }
+          slot.next(p.slots);
         }
         if (ok) commit_warp<CG>(smem_u32(&gb->acc_full[buf]));
+      }
+    }
+    __syncwarp();
+  } else if (warp == F4_SCALE_WARP) {
+    // ---------------- block scales: shared memory -> tensor memory, ahead of the MMAs ----------------
+    // A warp of its own: in the MMA issuer these copies and the wait for their slot sat between two steps' MMAs.
+    if (rank == 0) {
+      const uint32_t smem_base = __shfl_sync(0xffffffffu, smem_u32(smem), 0);
+      RingPos at, old, slot;  // `old`: the step whose scale slot is written next
+      bool ok = true, slots_used = false;
+      for (int tile = first; tile < p.num_tiles && ok; tile += step) {
+        for (int kb = 0; kb < p.k_steps; ++kb, at.next(stages)) {
+          // The slot's last readers are the MMAs of `slots` steps ago: they have retired when their stage is released.
+          if (slots_used) {
+            ok = __all_sync(0xffffffffu, bounded_wait(&gb->empty[old.stage], old.phase, &gb->abort_flag, status_word, 26));
+            if (!ok) break;
+            old.next(stages);
+          }
+          ok = __all_sync(0xffffffffu, bounded_wait(&gb->full[at.stage], at.phase, &gb->abort_flag, status_word, 27));
+          if (!ok) break;
+          tcgen05_fence_after();
+          const uint32_t base = smem_base + (uint32_t)at.stage * (uint32_t)p.stage_bytes;
+          const uint32_t sfa = tmem_base + p.sf_col + (uint32_t)slot.stage * SLOT_COLS;
+          const uint32_t sfb = sfa + TILES * 4;
+#pragma unroll
+          for (int j = 0; j < TILES; ++j) {
+            copy_scales<CG>(sfa + j * 4, scale_tile_desc(base + sfa_off + j * 512));
+#pragma unroll
+            for (int q = 0; q < PANELS; ++q)
+              copy_scales<CG>(sfb + (j * PANELS + q) * 4, scale_tile_desc(base + sfb_off + (q * TILES + j) * 512));
+          }
+          commit_own<CG>(smem_u32(&gb->sf_full[slot.stage]));
+          slot.next(p.slots);
+          slots_used = slots_used || slot.stage == 0;
+        }
       }
     }
     __syncwarp();
@@ -615,10 +648,15 @@ struct F4Plan {
 };
 // Tuning / testing knob: 0 = chosen by size, else the tile's columns, negative for a CTA pair's.
 static std::atomic<int> g_f4_tile{0};
-// Tile shape of a launch: the fewest waves of the cheapest tiles.  A step of a 256-column pair tile is the unit; costs
-// are relative clocks per step of 256 columns of K.
-static F4Plan f4_plan(int64_t M, int64_t N, int sms) {
-  const struct { bool pair; int bn; double step; } shapes[] = {{true, 256, 1.0}, {true, 128, 0.7}, {false, 128, 0.7}, {false, 64, 0.5}};
+// Tile shape of a launch, by a cost in steps of a 256-column pair tile (0.55 us): waves of tiles x steps x what a step
+// of that shape costs, plus what a launch of it costs whatever K (filling the ring, the last tile's epilogue).  Fitted
+// to nvfp4 launches with cold weights (M, N, K: 4608 x 5120 x 13824, 1153 x 12288 x 5120, 512 x 13824 x 5120, 77 x 5120
+// x 4096): pair 256 / pair 128 / single 128 / single 64 take 147 / 241 / 239 / 427, 51 / 59 / 60 / 105,
+// 30.2 / 29.2 / 29.4 / 51 and 16.1 / 12.1 / 11.3 / 10.7 us.
+static F4Plan f4_plan(int64_t M, int64_t N, int64_t K, int sms) {
+  const struct { bool pair; int bn; double step, launch; } shapes[] = {
+      {true, 256, 1.0, 15.0}, {true, 128, 0.82, 6.0}, {false, 128, 0.81, 5.5}, {false, 64, 0.72, 6.0}};
+  const int64_t k_steps = (K + FP4_STEP_COLS - 1) / FP4_STEP_COLS;
   const int forced = g_f4_tile.load(std::memory_order_relaxed);
   if (forced != 0) return F4Plan{forced < 0, forced < 0 ? -forced : forced};
   F4Plan best{true, 256};
@@ -628,7 +666,7 @@ static F4Plan f4_plan(int64_t M, int64_t N, int sms) {
     const int64_t bm = s.pair ? 256 : 128;
     const int64_t tiles = ((M + bm - 1) / bm) * ((N + s.bn - 1) / s.bn);
     const int64_t slots = s.pair ? sms / 2 : sms;
-    const double cost = (double)((tiles + slots - 1) / slots) * s.step;
+    const double cost = (double)((tiles + slots - 1) / slots * k_steps) * s.step + s.launch;
     if (cost < best_cost) {
       best_cost = cost;
       best = F4Plan{s.pair, s.bn};
@@ -700,7 +738,7 @@ static int f4_gemm(const F4Matrix& a, const F4Matrix& w, const void* bias, void*
                    int64_t ld_out, int gelu, int32_t* status_word, cudaStream_t st) {
   if (g_f4_tile.load(std::memory_order_relaxed) == 0 && M <= F4V_MAX_M && M * f4v_row_bytes((int)((K + 63) / 64)) <= F4V_SMEM_LIMIT)
     return f4_gemv<NV, T>(a, w, bias, out, M, N, K, ld_out, gelu, st);
-  const F4Plan plan = f4_plan(M, N, sm_count());
+  const F4Plan plan = f4_plan(M, N, K, sm_count());
   const int cg = plan.pair ? 2 : 1, bn = plan.bn;
   const int panels = bn > 128 ? bn / 128 : 1;
   F4Params p{};
@@ -730,11 +768,10 @@ static int f4_gemm(const F4Matrix& a, const F4Matrix& w, const void* bias, void*
   p.stage_bytes = F4_A_BYTES + bn / cg * 128 + (NV ? 4 : 2) * 512 * (1 + panels);
   const int fit = (F4_SMEM_LIMIT - F4_FIXED_BYTES) / p.stage_bytes;
   p.stages = fit < F4_MAX_STAGES ? fit : F4_MAX_STAGES;
-  // Scale slots: what the accumulators leave of tensor memory, and no more than stages.  The MMA issuer tells a slot's
-  // release by its stage's barrier, whose phase bit says nothing about a use more than one round of the ring ago.
+  // Scale slots: what the accumulators leave of tensor memory, and no more than stages.  A slot's release is told by its stage's barrier, whose phase bit says nothing about a use more than one round of the ring ago.
   p.sf_col = bn == F4_MAX_BN ? F4_SHARED_COL + F4_MAX_BN : 2 * bn;
   const uint32_t fit_slots = (F4_TMEM_COLS - p.sf_col) / ((NV ? 16 : 8) * (1 + panels));
-  p.slots = fit_slots < (uint32_t)p.stages ? fit_slots : (uint32_t)p.stages;
+  p.slots = (int)fit_slots < p.stages ? (int)fit_slots : p.stages;
   if (plan.pair) return bn == 256 ? f4_launch<2, 256, NV, T>(p, status_word, st) : f4_launch<2, 128, NV, T>(p, status_word, st);
   return bn == 128 ? f4_launch<1, 128, NV, T>(p, status_word, st) : f4_launch<1, 64, NV, T>(p, status_word, st);
 }

@@ -160,3 +160,41 @@ def test_linear_bias_and_gelu(m, n, k, gelu, dtype, fmt):
   got = cd.float4_linear(x, cd.float4_quantize_rows(w.cuda(), fmt), bias.cuda(), gelu=gelu)
   assert got.shape == (1, m, n) and got.dtype == dtype
   assert (np.abs(got[0].double().cpu().numpy() - want) <= bound).all()
+
+
+TILES = [(0, 64), (0, 128), (1, 128), (1, 256)]
+
+
+@pytest.fixture
+def tile(request):
+  pair, cols = request.param
+  assert _native.lib().cdb_tuning_set_fp4_tile(pair, cols) == 0
+  yield request.param
+  assert _native.lib().cdb_tuning_set_fp4_tile(0, 0) == 0
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("tile", TILES, indirect=True)
+@pytest.mark.parametrize("m,n,k", [(3, 8, 32), (130, 200, 288), (257, 264, 1312), (300, 720, 2048)])
+def test_every_tile_shape(m, n, k, tile, fmt):
+  qa, qw, va, vw = _operands(m, n, k, fmt, m + n + k)
+  y = va @ vw.T
+  got = cd.float4_scaled_mm(qa, qw).double().cpu().numpy()
+  assert (np.abs(got - y) <= _product_bound(va, vw, y, k, torch.bfloat16)).all()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("tile", TILES, indirect=True)
+def test_many_tiles_per_cta(tile, fmt):
+  """More tiles than SMs, so every CTA goes round its accumulators, scale slots and ring several times."""
+  m, n, k = 3500, 8200, 1056
+  g = torch.Generator().manual_seed(1)
+  a, w = (torch.randn(r, k, generator=g).cuda() for r in (m, n))
+  qa, qw = cd.float4_quantize_rows(a, fmt), cd.float4_quantize_rows(w, fmt)
+  va, vw = (cd.float4_dequantize_rows(q, torch.float32).double() for q in (qa, qw))
+  y = va @ vw.t()
+  bound = (k / 16 + 4) * 2.0**-23 * (va.abs() @ vw.abs().t() + y.abs()) + 2.0**-8 * y.abs() + 1e-30
+  for _ in range(3):
+    got = cd.float4_scaled_mm(qa, qw).double()
+    assert ((got - y).abs() <= bound).all()
+  assert _native.gemm_device_status(torch.device("cuda")) == 0
