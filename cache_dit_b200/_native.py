@@ -54,6 +54,7 @@ SIGNATURES = {
   "cdb_fp4_gemm": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int, c_int, c_int,
                            c_void_p, c_void_p]),
   "cdb_tuning_set_fp4_tile": (c_int, [c_int, c_int]),
+  "cdb_gated_residual_norm": (c_int, [c_void_p, c_int, c_void_p]),
   "cdb_qk_norm_rope": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64,
                                c_int64, c_int64, c_int, c_int, c_int, c_float, c_void_p]),
   "cdb_gated_residual_pair": (c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64,
@@ -702,3 +703,45 @@ def fp4_gemm(a, w, bias, out, cols: int, fmt: str, gelu: bool = False):
                             out.stride(0) if M > 1 else N, FP4_FORMATS[fmt], DTYPE_ID[out.dtype], int(gelu),
                             _ptr(gemm_status_word(out.device)), _stream(out))
   check(st, "cdb_fp4_gemm")
+
+
+# ---- gated residual with norms -------------------------------------------------------------------
+NORM_KINDS = {None: 0, "rms": 1, "layer": 2}
+NORM_MAX_DIM = 16384
+
+
+class NormArgs(ctypes.Structure):
+  """ctypes image of `cdb_norm_args`."""
+  _fields_ = [(n, c_void_p) for n in ("x", "y", "gate", "post_weight", "post_bias", "weight", "bias", "scale", "shift")] + \
+      [(n, c_int64) for n in ("x_batch", "x_row", "y_batch", "y_row", "gate_batch", "scale_batch", "shift_batch")] + \
+      [(n, c_void_p) for n in ("x_out", "h_out", "codes", "block_scales", "row_scale")] + \
+      [(n, c_int64) for n in ("batch", "tokens", "dim")] + [(n, c_int) for n in ("post", "norm", "format")] + \
+      [(n, c_float) for n in ("residual_scale", "post_eps", "eps")]
+
+
+def gated_residual_norm(x, y, vectors, x_out, h_out, fp4, post, norm, residual_scale: float, post_eps: float, eps: float):
+  """x, y [batch, tokens, dim] with unit column stride (y may be None); `vectors`: gate, post_weight, post_bias, weight,
+  bias, scale, shift by name ([dim], or [batch, dim] for gate / scale / shift; None or missing: absent); h goes to h_out or,
+  as (codes, block_scales, row_scale, format), to `fp4` (see cdb_gated_residual_norm)."""
+  a = NormArgs()
+  a.batch, a.tokens, a.dim = x.shape
+  a.x, a.x_batch, a.x_row = x.data_ptr(), x.stride(0), x.stride(1)
+  if y is not None:
+    a.y, a.y_batch, a.y_row = y.data_ptr(), y.stride(0), y.stride(1)
+    a.x_out = x_out.data_ptr()
+  for name, t in vectors.items():
+    if t is not None:
+      setattr(a, name, t.data_ptr())
+      if t.dim() == 2:
+        setattr(a, name + "_batch", t.stride(0))
+  a.h_out = None if h_out is None else h_out.data_ptr()
+  a.format = -1
+  if fp4 is not None:
+    codes, block_scales, row_scale, fmt = fp4
+    a.codes, a.block_scales, a.format = codes.data_ptr(), block_scales.data_ptr(), FP4_FORMATS[fmt]
+    a.row_scale = None if row_scale is None else row_scale.data_ptr()
+  a.post, a.norm = NORM_KINDS[post], NORM_KINDS[norm]
+  a.residual_scale, a.post_eps, a.eps = residual_scale, post_eps, eps
+  with torch.cuda.device(x.device):
+    st = lib().cdb_gated_residual_norm(ctypes.byref(a), DTYPE_ID[x.dtype], _stream(x))
+  check(st, "cdb_gated_residual_norm")

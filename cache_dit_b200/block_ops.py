@@ -1,0 +1,99 @@
+"""Operators of transformer blocks around the linears: a gated residual with norms on either side, and attention to an
+encoder's states.
+
+In the models the reference wraps these are eager PyTorch ops inside the diffusers blocks.  Inference only: inputs that
+ask for gradients are refused.  All tensors of a call lie on one CUDA device; results are new, contiguous tensors on the
+current stream of that device.
+"""
+from __future__ import annotations
+
+from typing import Optional, Tuple, Union
+
+import torch
+
+from . import _native
+from .quantization.float4 import FORMATS, Float4Rows, empty_rows, no_gradients, one_device
+
+_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
+
+
+def _rows_of(what: str, name: str, t: torch.Tensor, shape, dtype) -> torch.Tensor:
+  if tuple(t.shape) != tuple(shape) or t.dtype != dtype:
+    raise RuntimeError(f"{what}: {name} must be {dtype} {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+  t = t if t.dim() == 3 else t.reshape(1, -1, t.shape[-1])
+  return t if t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous()
+
+
+def _vector_of(what: str, name: str, t: Optional[torch.Tensor], batch: int, dim: int, dtype, per_batch: bool):
+  if t is None:
+    return None
+  shapes = [(dim, )] + ([(batch, dim), (1, dim)] if per_batch else [])
+  if t.dtype != dtype or tuple(t.shape) not in shapes:
+    raise RuntimeError(f"{what}: {name} must be {dtype} {' or '.join(map(str, shapes[:2]))}, got {t.dtype} {tuple(t.shape)}")
+  if t.dim() == 2 and t.shape[0] == 1 and batch != 1:
+    t = t[0]
+  return t if t.stride(-1) == 1 or dim == 1 else t.contiguous()
+
+
+def gated_residual_norm(x: torch.Tensor, y: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None, *,
+                        residual_scale: float = 1.0, post_norm: Optional[str] = None,
+                        post_weight: Optional[torch.Tensor] = None, post_bias: Optional[torch.Tensor] = None,
+                        post_eps: float = 1e-6, norm: Optional[str] = "layer", weight: Optional[torch.Tensor] = None,
+                        bias: Optional[torch.Tensor] = None, scale: Optional[torch.Tensor] = None,
+                        shift: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                        quantize: Optional[str] = None) -> Tuple[torch.Tensor, Union[torch.Tensor, Float4Rows, None]]:
+  """(x', h) in one pass over the rows:
+
+      x' = x + residual_scale * gate * post_norm(y)
+      h  = norm(x') * weight + bias, then * (1 + scale) + shift
+
+  x, y [batch, tokens, dim] (or [rows, dim]: one batch) in float32, bfloat16 or float16; rows may be strided.  The norms
+  are "rms", "layer" or None (post_norm: y as it is; norm: no h).  gate, scale and shift are [batch, dim] or [dim],
+  weights and biases [dim], all in x's type.  Without y, x' is x itself and only the norm runs.
+  quantize = "nvfp4" | "mxfp4": h comes back as `Float4Rows`, the 4-bit form of exactly the h that would be returned
+  without it; dim must then be a multiple of 32.  The norm reads x' before its rounding to x's type."""
+  what = "gated_residual_norm"
+  if x.dtype not in _DTYPES or x.dim() not in (2, 3):
+    raise RuntimeError(f"{what}: x must be [batch, tokens, dim] or [rows, dim] in float32, bfloat16 or float16, got "
+                       f"{x.dtype} {tuple(x.shape)}")
+  for name, kind in (("post_norm", post_norm), ("norm", norm)):
+    if kind not in _native.NORM_KINDS:
+      raise ValueError(f"{what}: {name} must be 'rms', 'layer' or None, not {kind!r}")
+  if y is None and (gate is not None or post_norm is not None or residual_scale != 1.0):
+    raise RuntimeError(f"{what}: gate, post_norm and residual_scale belong to y, which is missing")
+  if post_norm is None and (post_weight is not None or post_bias is not None):
+    raise RuntimeError(f"{what}: post_weight and post_bias belong to post_norm, which is None")
+  if norm is None and (y is None or any(t is not None for t in (weight, bias, scale, shift)) or quantize is not None):
+    raise RuntimeError(f"{what}: without norm there is nothing but x' to compute")
+  if (scale is None) != (shift is None):
+    raise RuntimeError(f"{what}: scale and shift go together")
+  dim = x.shape[-1]
+  if dim == 0 or dim > _native.NORM_MAX_DIM:
+    raise RuntimeError(f"{what}: rows of 1 to {_native.NORM_MAX_DIM} elements, got {dim}")
+  if quantize is not None:
+    if quantize not in FORMATS:
+      raise ValueError(f"{what}: unknown 4-bit format {quantize!r}; supported: {FORMATS}")
+    if dim % 32 != 0:
+      raise RuntimeError(f"{what}: 4-bit rows need a width that is a multiple of 32, got {dim}")
+  tensors = dict(x=x, y=y, gate=gate, post_weight=post_weight, post_bias=post_bias, weight=weight, bias=bias, scale=scale, shift=shift)
+  one_device(what, *tensors.values())
+  no_gradients(what, *tensors.values())
+  batch = x.shape[0] if x.dim() == 3 else 1
+  x3 = _rows_of(what, "x", x, x.shape, x.dtype)
+  y3 = None if y is None else _rows_of(what, "y", y, x.shape, x.dtype)
+  vectors = {name: _vector_of(what, name, tensors[name], batch, dim, x.dtype, name in ("gate", "scale", "shift"))
+             for name in ("gate", "post_weight", "post_bias", "weight", "bias", "scale", "shift")}
+  x_out = x if y is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+  h = None
+  if quantize is not None:
+    h = empty_rows(x.shape[:-1], dim, quantize, x.device)
+    aligned = lambda t: t is None or (t.data_ptr() % 16 == 0 and all(s * t.element_size() % 16 == 0 for s in t.stride()[:-1]))
+    x3, y3 = (t if aligned(t) else t.clone(memory_format=torch.contiguous_format) for t in (x3, y3))
+    vectors = {name: t if aligned(t) else t.clone(memory_format=torch.contiguous_format) for name, t in vectors.items()}
+  elif norm is not None:
+    h = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+  if x.numel():
+    _native.gated_residual_norm(x3, y3, vectors, x_out, h if quantize is None else None,
+                                None if quantize is None else (*h._triple(), quantize), post_norm, norm,
+                                float(residual_scale), float(post_eps), float(eps))
+  return x_out, h

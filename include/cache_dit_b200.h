@@ -393,6 +393,30 @@ CDB_API int cdb_fp4_gemm(const void* a /* cdb_fp4_matrix */, const void* w /* cd
  * by size; pair = 0: one SM, 128 x cols, cols 64 or 128; pair = 1: a pair of SMs, 256 x cols, cols 128 or 256. */
 CDB_API int cdb_tuning_set_fp4_tile(int pair, int cols);
 
+/* ------------------------------------------------------------------------------------------
+ * Gated residual with a norm before and after it (no counterpart in the reference: eager PyTorch ops inside the
+ * diffusers blocks).  Per row of [batch, tokens, dim]:
+ *   x_out = x + residual_scale * gate[b] * post(y)      post: 0 none, 1 RMSNorm, 2 LayerNorm, * post_weight + post_bias
+ *   h     = norm(x_out before rounding) * weight + bias, then * (1 + scale[b]) + shift[b]   norm: 0 none, 1 RMS, 2 Layer
+ * computed in fp32, each output rounded once.  format = -1: h_out in the tensors' type; CDB_NVFP4 / CDB_MXFP4: the 4-bit
+ * form of that very h (see cdb_fp4_quant_rows) into codes / block_scales / row_scale.
+ * All tensors are `dtype` with unit column stride; x and y have batch and row strides in elements, gate / scale / shift
+ * a batch stride (0: one vector for all), weights are [dim]; outputs are contiguous.  NULL: y (then x_out, gate and post
+ * are absent too: only the norm), gate, weights, biases, scale with shift.  Any dim up to CDB_NORM_MAX_DIM; 4-bit output
+ * needs dim % 32 == 0 and everything 16-byte aligned; elsewhere alignment only costs speed.
+ * ---------------------------------------------------------------------------------------- */
+#define CDB_NORM_MAX_DIM 16384
+typedef struct cdb_norm_args {
+  const void *x, *y, *gate, *post_weight, *post_bias, *weight, *bias, *scale, *shift;
+  int64_t x_batch, x_row, y_batch, y_row, gate_batch, scale_batch, shift_batch;
+  void *x_out, *h_out, *codes, *block_scales;
+  float* row_scale;
+  int64_t batch, tokens, dim;
+  int post, norm, format;
+  float residual_scale, post_eps, eps;
+} cdb_norm_args;
+CDB_API int cdb_gated_residual_norm(const void* args /* cdb_norm_args */, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
