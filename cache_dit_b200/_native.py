@@ -55,6 +55,9 @@ SIGNATURES = {
                            c_void_p, c_void_p]),
   "cdb_tuning_set_fp4_tile": (c_int, [c_int, c_int]),
   "cdb_gated_residual_norm": (c_int, [c_void_p, c_int, c_void_p]),
+  "cdb_cross_attention_workspace_bytes": (c_size_t, [c_int64] * 6 + [c_int]),
+  "cdb_cross_attention": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p] + [c_int64] * 6 +
+                          [c_float, c_int, c_void_p, c_size_t, c_void_p, c_void_p]),
   "cdb_qk_norm_rope": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64,
                                c_int64, c_int64, c_int, c_int, c_int, c_float, c_void_p]),
   "cdb_gated_residual_pair": (c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64,
@@ -745,3 +748,27 @@ def gated_residual_norm(x, y, vectors, x_out, h_out, fp4, post, norm, residual_s
   with torch.cuda.device(x.device):
     st = lib().cdb_gated_residual_norm(ctypes.byref(a), DTYPE_ID[x.dtype], _stream(x))
   check(st, "cdb_gated_residual_norm")
+
+
+# ---- cross attention -----------------------------------------------------------------------------
+CROSS_MAX_HEAD_DIM = 128
+
+
+class Heads(ctypes.Structure):
+  """ctypes image of `cdb_heads`."""
+  _fields_ = [("data", c_void_p), ("batch_stride", c_int64), ("token_stride", c_int64), ("head_stride", c_int64)]
+
+
+def cross_attention(q, k, v, key_mask, scale: float, out):
+  """q [b, sq, h, d], k / v [b, skv, kv_h, d] with unit stride within a head, key_mask bool [b, skv] or None, out
+  contiguous like q (see cdb_cross_attention).  The workspace belongs to this call."""
+  b, sq, h, d = q.shape
+  skv, kv_h = k.shape[1], k.shape[2]
+  qh, kh, vh = (Heads(t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)) for t in (q, k, v))
+  with torch.cuda.device(q.device):
+    need = lib().cdb_cross_attention_workspace_bytes(b, sq, skv, h, kv_h, d, int(key_mask is not None))
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    st = lib().cdb_cross_attention(ctypes.byref(qh), ctypes.byref(kh), ctypes.byref(vh), _ptr(key_mask),
+                                   0 if key_mask is None else key_mask.stride(0), _ptr(out), b, sq, skv, h, kv_h, d, scale,
+                                   DTYPE_ID[q.dtype], _ptr(ws), need, _ptr(gemm_status_word(q.device)), _stream(q))
+  check(st, "cdb_cross_attention")

@@ -7,6 +7,7 @@ current stream of that device.
 """
 from __future__ import annotations
 
+import math
 from typing import Optional, Tuple, Union
 
 import torch
@@ -97,3 +98,48 @@ def gated_residual_norm(x: torch.Tensor, y: Optional[torch.Tensor] = None, gate:
                                 None if quantize is None else (*h._triple(), quantize), post_norm, norm,
                                 float(residual_scale), float(post_eps), float(eps))
   return x_out, h
+
+
+def _heads_of(t: torch.Tensor) -> torch.Tensor:
+  """t [batch, tokens, heads, d] as the kernel's loads want it: unit stride within a head, every other stride positive and a
+  multiple of 16 bytes, base 16-byte aligned; copied only where it is not."""
+  ok = t.data_ptr() % 16 == 0 and (t.stride(3) == 1 or t.shape[3] == 1) and \
+      all(n == 1 or (s > 0 and s % 8 == 0) for n, s in zip(t.shape[:3], t.stride()[:3]))
+  return t if ok else t.clone(memory_format=torch.contiguous_format)
+
+
+def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, key_mask: Optional[torch.Tensor] = None,
+                    scale: Optional[float] = None) -> torch.Tensor:
+  """softmax(scale * q k^T) v for q [batch, tokens, heads, d] and an encoder's k, v [batch, keys, kv_heads, d], in bfloat16
+  or float16; heads is a multiple of kv_heads, consecutive query heads share a key / value head; d a multiple of 8, at
+  most 128.  key_mask bool [batch, keys]: True keeps the key; a batch entry that keeps none gives zeros, and what lies in
+  masked places of k and v (infinities and NaN too) has no effect.  scale defaults to 1 / sqrt(d).
+  Returns [batch, tokens, heads, d]."""
+  what = "cross_attention"
+  if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
+    raise RuntimeError(f"{what}: q [batch, tokens, heads, d] and k, v [batch, keys, kv_heads, d], got {tuple(q.shape)}, "
+                       f"{tuple(k.shape)}, {tuple(v.shape)}")
+  if q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
+    raise RuntimeError(f"{what}: q, k and v must all be bfloat16 or all float16, got {q.dtype}, {k.dtype}, {v.dtype}")
+  b, sq, h, d = q.shape
+  skv, kv_h = k.shape[1], k.shape[2]
+  if h == 0 or kv_h == 0 or h % kv_h != 0:
+    raise RuntimeError(f"{what}: the number of query heads ({h}) must be a multiple of the key heads ({kv_h})")
+  if d == 0 or d % 8 != 0 or d > _native.CROSS_MAX_HEAD_DIM:
+    raise RuntimeError(f"{what}: the head dimension must be a multiple of 8 and at most {_native.CROSS_MAX_HEAD_DIM}, got {d}")
+  if key_mask is not None and (key_mask.dtype != torch.bool or tuple(key_mask.shape) != (b, skv)):
+    raise RuntimeError(f"{what}: key_mask must be bool {(b, skv)}, got {key_mask.dtype} {tuple(key_mask.shape)}")
+  scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
+  if not (scale > 0.0 and math.isfinite(scale)):
+    raise RuntimeError(f"{what}: scale must be positive and finite, got {scale}")
+  one_device(what, q, k, v, key_mask)
+  no_gradients(what, q, k, v)
+  out = torch.empty((b, sq, h, d), dtype=q.dtype, device=q.device)
+  if out.numel() == 0:
+    return out
+  if skv == 0:
+    return out.zero_()
+  if key_mask is not None and key_mask.stride(1) != 1 and skv > 1:
+    key_mask = key_mask.contiguous()
+  _native.cross_attention(_heads_of(q), _heads_of(k), _heads_of(v), key_mask, scale, out)
+  return out

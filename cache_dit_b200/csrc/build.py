@@ -17,7 +17,7 @@ PKG = os.path.dirname(HERE)
 LIB_NAME = "libcache_dit_b200.so"
 LIB_PATH = os.path.join(PKG, LIB_NAME)
 SOURCES = ["lib.cu", "cache_kernels.cu", "fp8_quant.cu", "fp8_gemm.cu", "glue_kernels.cu", "peer_kernels.cu",
-           "fp4_quant.cu", "fp4_gemm.cu", "norm_kernels.cu"]
+           "fp4_quant.cu", "fp4_gemm.cu", "norm_kernels.cu", "cross_attention.cu"]
 HEADERS = ["common.cuh", "tcgen05.cuh", "fp4.cuh", os.path.join("..", "..", "include", "cache_dit_b200.h")]
 NVCC_FLAGS = [
   "-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-std=c++17", "-lineinfo",

@@ -417,6 +417,30 @@ typedef struct cdb_norm_args {
 } cdb_norm_args;
 CDB_API int cdb_gated_residual_norm(const void* args /* cdb_norm_args */, int dtype, void* stream);
 
+/* ------------------------------------------------------------------------------------------
+ * Attention of tokens to an encoder's states of another length (in the reference a call of an attention backend inside
+ * the diffusers blocks):
+ *   out[b, s, h] = sum_t softmax_t(scale * q[b, s, h] . k[b, t, h / G]) v[b, t, h / G]     over the kept keys t
+ * q [batch, sq, heads, d], k and v [batch, skv, kv_heads, d], heads = G * kv_heads, `dtype` CDB_BF16 or CDB_F16, unit
+ * stride within a head; the other strides (elements) are multiples of 8, pointers 16-byte aligned; d % 8 == 0, at most
+ * CDB_CROSS_MAX_HEAD_DIM.  out [batch, sq, heads, d] contiguous.  key_mask: one byte per key, rows ld_mask bytes apart,
+ * non-zero = kept; NULL keeps all.  A batch entry without a kept key gives zeros; values in masked places of k and v
+ * (NaN too) have no effect.  scale > 0.
+ * `workspace`: cdb_cross_attention_workspace_bytes() for the current device, 16-byte aligned, not zeroed, in use until the
+ * call's work is done.  `status_word` as in cdb_fp8_gemm_rowscaled.
+ * ---------------------------------------------------------------------------------------- */
+#define CDB_CROSS_MAX_HEAD_DIM 128
+typedef struct cdb_heads {
+  const void* data;
+  int64_t batch_stride, token_stride, head_stride;
+} cdb_heads;
+CDB_API size_t cdb_cross_attention_workspace_bytes(int64_t batch, int64_t sq, int64_t skv, int64_t heads, int64_t kv_heads,
+                                                   int64_t d, int masked);
+CDB_API int cdb_cross_attention(const void* q /* cdb_heads */, const void* k, const void* v, const void* key_mask,
+                                int64_t ld_mask, void* out, int64_t batch, int64_t sq, int64_t skv, int64_t heads,
+                                int64_t kv_heads, int64_t d, float scale, int dtype, void* workspace,
+                                size_t workspace_bytes, int32_t* status_word, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
