@@ -53,6 +53,9 @@ SIGNATURES = {
   "cdb_fp4_dequant_rows": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int, c_void_p, c_int, c_void_p]),
   "cdb_fp4_gemm": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int, c_int, c_int,
                            c_void_p, c_void_p]),
+  "cdb_fp4_linear_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int]),
+  "cdb_fp4_linear": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int, c_int,
+                             c_int, c_void_p, c_size_t, c_void_p, c_void_p]),
   "cdb_tuning_set_fp4_tile": (c_int, [c_int, c_int]),
   "cdb_gated_residual_norm": (c_int, [c_void_p, c_int, c_void_p]),
   "cdb_cross_attention_workspace_bytes": (c_size_t, [c_int64] * 6 + [c_int]),
@@ -664,6 +667,37 @@ def gated_residual_pair(xa, gate_a, ya, xb, gate_b, yb):
   return outs[0], outs[1]
 
 
+# ---- launching without ceremony --------------------------------------------------------------------
+# The operators below are called for a handful of tokens too, where a kernel takes a few microseconds: their wrappers
+# pass plain integers and touch the current device only when the tensors lie on another one.
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_status_ptrs = {}
+
+
+def _status_ptr(index: int) -> int:
+  p = _status_ptrs.get(index)
+  if p is None:
+    p = _status_ptrs[index] = gemm_status_word(torch.device("cuda", index)).data_ptr()  # the mailbox is never freed
+  return p
+
+
+def _on_device(index: int, fn, what: str, *args):
+  """fn(*args, stream) with the tensors' device current, on its current stream."""
+  global launch_count
+  if index == torch.cuda.current_device():
+    st = fn(*args, _raw_stream(index))
+  else:
+    with torch.cuda.device(index):
+      st = fn(*args, _raw_stream(index))
+  launch_count += 1
+  if st != 0:
+    check(st, what, launch=False)
+
+
+def _dp(t):
+  return None if t is None else t.data_ptr()
+
+
 # ---- 4-bit microscaled matrices ------------------------------------------------------------------
 FP4_FORMATS = {"nvfp4": 0, "mxfp4": 1}
 FP4_BLOCK = {"nvfp4": 16, "mxfp4": 32}
@@ -677,35 +711,38 @@ class Fp4Matrix(ctypes.Structure):
 
 def fp4_block_scale_bytes(rows: int, cols: int, fmt: str) -> int:
   """Bytes of the tiled block scales of a [rows, cols] matrix (host arithmetic only)."""
-  tiles = -(-cols // 256) * (256 // FP4_BLOCK[fmt]) // 4
-  return -(-rows // 128) * tiles * 512
+  return -(-rows // 128) * -(-cols // 256) * (8192 if fmt == "nvfp4" else 4096) // 4
 
 
-def fp4_quant_rows(x2d, codes, block_scales, row_scale, fmt: str):
-  """x2d [rows, cols] f32 / bf16 / f16 (rows may be strided) -> 4-bit codes and scales (see cdb_fp4_quant_rows)."""
-  rows, cols = x2d.shape
-  with torch.cuda.device(x2d.device):
-    st = lib().cdb_fp4_quant_rows(_ptr(x2d), rows, cols, x2d.stride(0) if rows > 1 else cols, DTYPE_ID[x2d.dtype],
-                                  FP4_FORMATS[fmt], _ptr(codes), _ptr(block_scales), _ptr(row_scale), _stream(x2d))
-  check(st, "cdb_fp4_quant_rows")
+def fp4_quant_rows(x, ld_x: int, rows: int, cols: int, codes, block_scales, row_scale, fmt: str):
+  """x: `rows` rows of `cols` f32 / bf16 / f16 elements, ld_x apart -> 4-bit codes and scales (see cdb_fp4_quant_rows)."""
+  _on_device(x.device.index, lib().cdb_fp4_quant_rows, "cdb_fp4_quant_rows", x.data_ptr(), rows, cols, ld_x, DTYPE_ID[x.dtype], FP4_FORMATS[fmt], codes.data_ptr(),
+             block_scales.data_ptr(), _dp(row_scale))
 
 
-def fp4_dequant_rows(codes, block_scales, row_scale, cols: int, fmt: str, out):
-  with torch.cuda.device(out.device):
-    st = lib().cdb_fp4_dequant_rows(_ptr(codes), _ptr(block_scales), _ptr(row_scale), out.shape[0], cols, FP4_FORMATS[fmt],
-                                    _ptr(out), DTYPE_ID[out.dtype], _stream(out))
-  check(st, "cdb_fp4_dequant_rows")
+def fp4_dequant_rows(codes, block_scales, row_scale, rows: int, cols: int, fmt: str, out):
+  _on_device(out.device.index, lib().cdb_fp4_dequant_rows, "cdb_fp4_dequant_rows", codes.data_ptr(), block_scales.data_ptr(),
+             _dp(row_scale), rows, cols, FP4_FORMATS[fmt], out.data_ptr(), DTYPE_ID[out.dtype])
 
 
-def fp4_gemm(a, w, bias, out, cols: int, fmt: str, gelu: bool = False):
-  """out [M, N] = act(a [M, cols] @ w [N, cols]^T + bias) for two (codes, block_scales, row_scale) triples (see cdb_fp4_gemm)."""
-  M, N = out.shape
-  am, wm = (Fp4Matrix(*[None if t is None else t.data_ptr() for t in triple]) for triple in (a, w))
-  with torch.cuda.device(out.device):
-    st = lib().cdb_fp4_gemm(ctypes.byref(am), ctypes.byref(wm), _ptr(bias), _ptr(out), M, N, cols,
-                            out.stride(0) if M > 1 else N, FP4_FORMATS[fmt], DTYPE_ID[out.dtype], int(gelu),
-                            _ptr(gemm_status_word(out.device)), _stream(out))
-  check(st, "cdb_fp4_gemm")
+def fp4_gemm(a, w, bias, out, rows: int, cols: int, fmt: str, gelu: bool = False):
+  """out [rows, N] (contiguous, any leading shape) = act(a [rows, cols] @ w [N, cols]^T + bias) for two (codes, block_scales,
+  row_scale) triples (see cdb_fp4_gemm)."""
+  n = out.shape[-1]
+  index = out.device.index
+  _on_device(index, lib().cdb_fp4_gemm, "cdb_fp4_gemm", ctypes.byref(Fp4Matrix(*map(_dp, a))), ctypes.byref(Fp4Matrix(*map(_dp, w))),
+             _dp(bias), out.data_ptr(), rows, n, cols, n, FP4_FORMATS[fmt], DTYPE_ID[out.dtype], int(gelu), _status_ptr(index))
+
+
+def fp4_linear(x, ld_x: int, w, bias, out, rows: int, cols: int, fmt: str, gelu: bool):
+  """out [rows, N] = act(x [rows, cols] @ w [N, cols]^T + bias), x quantised on the way (see cdb_fp4_linear)."""
+  n = out.shape[-1]
+  index = out.device.index
+  f = FP4_FORMATS[fmt]
+  need = (rows * (cols >> 1) + 255) // 256 * 256 + fp4_block_scale_bytes(rows, cols, fmt) + rows * 4
+  ws = torch.empty(need, dtype=torch.uint8, device=out.device)
+  _on_device(index, lib().cdb_fp4_linear, "cdb_fp4_linear", x.data_ptr(), ld_x, ctypes.byref(Fp4Matrix(*map(_dp, w))), _dp(bias),
+             out.data_ptr(), rows, n, cols, n, f, DTYPE_ID[out.dtype], int(gelu), ws.data_ptr(), need, _status_ptr(index))
 
 
 # ---- gated residual with norms -------------------------------------------------------------------
@@ -722,32 +759,23 @@ class NormArgs(ctypes.Structure):
       [(n, c_float) for n in ("residual_scale", "post_eps", "eps")]
 
 
-def gated_residual_norm(x, y, vectors, x_out, h_out, fp4, post, norm, residual_scale: float, post_eps: float, eps: float):
-  """x, y [batch, tokens, dim] with unit column stride (y may be None); `vectors`: gate, post_weight, post_bias, weight,
-  bias, scale, shift by name ([dim], or [batch, dim] for gate / scale / shift; None or missing: absent); h goes to h_out or,
-  as (codes, block_scales, row_scale, format), to `fp4` (see cdb_gated_residual_norm)."""
-  a = NormArgs()
-  a.batch, a.tokens, a.dim = x.shape
-  a.x, a.x_batch, a.x_row = x.data_ptr(), x.stride(0), x.stride(1)
-  if y is not None:
-    a.y, a.y_batch, a.y_row = y.data_ptr(), y.stride(0), y.stride(1)
-    a.x_out = x_out.data_ptr()
-  for name, t in vectors.items():
-    if t is not None:
-      setattr(a, name, t.data_ptr())
-      if t.dim() == 2:
-        setattr(a, name + "_batch", t.stride(0))
-  a.h_out = None if h_out is None else h_out.data_ptr()
-  a.format = -1
-  if fp4 is not None:
-    codes, block_scales, row_scale, fmt = fp4
-    a.codes, a.block_scales, a.format = codes.data_ptr(), block_scales.data_ptr(), FP4_FORMATS[fmt]
-    a.row_scale = None if row_scale is None else row_scale.data_ptr()
-  a.post, a.norm = NORM_KINDS[post], NORM_KINDS[norm]
-  a.residual_scale, a.post_eps, a.eps = residual_scale, post_eps, eps
-  with torch.cuda.device(x.device):
-    st = lib().cdb_gated_residual_norm(ctypes.byref(a), DTYPE_ID[x.dtype], _stream(x))
-  check(st, "cdb_gated_residual_norm")
+def _batch_stride(t) -> int:
+  return 0 if t is None or t.dim() == 1 else t.stride(0)
+
+
+def gated_residual_norm(x, y, gate, post_weight, post_bias, weight, bias, scale, shift, x_out, h_out, fp4, post, norm,
+                        residual_scale: float, post_eps: float, eps: float):
+  """x, y [batch, tokens, dim] with unit column stride (y may be None); gate, scale, shift [dim] or [batch, dim], weights and
+  biases [dim], None: absent; h goes to h_out or, as (codes, block_scales, row_scale, format), to `fp4` (see
+  cdb_gated_residual_norm)."""
+  b, t, dim = x.shape
+  codes, block_scales, row_scale, fmt = (None, None, None, -1) if fp4 is None else (*map(_dp, fp4[:3]), FP4_FORMATS[fp4[3]])
+  yb, yt = (0, 0) if y is None else (y.stride(0), y.stride(1))
+  a = NormArgs(x.data_ptr(), _dp(y), _dp(gate), _dp(post_weight), _dp(post_bias), _dp(weight), _dp(bias), _dp(scale), _dp(shift),
+               x.stride(0), x.stride(1), yb, yt, _batch_stride(gate), _batch_stride(scale), _batch_stride(shift),
+               None if y is None else x_out.data_ptr(), _dp(h_out), codes, block_scales, row_scale, b, t, dim, NORM_KINDS[post],
+               NORM_KINDS[norm], fmt, residual_scale, post_eps, eps)
+  _on_device(x.device.index, lib().cdb_gated_residual_norm, "cdb_gated_residual_norm", ctypes.byref(a), DTYPE_ID[x.dtype])
 
 
 # ---- cross attention -----------------------------------------------------------------------------
@@ -759,16 +787,22 @@ class Heads(ctypes.Structure):
   _fields_ = [("data", c_void_p), ("batch_stride", c_int64), ("token_stride", c_int64), ("head_stride", c_int64)]
 
 
+def _workspace_bytes_on(index: int, *args) -> int:
+  if index == torch.cuda.current_device():
+    return lib().cdb_cross_attention_workspace_bytes(*args)
+  with torch.cuda.device(index):
+    return lib().cdb_cross_attention_workspace_bytes(*args)
+
+
 def cross_attention(q, k, v, key_mask, scale: float, out):
   """q [b, sq, h, d], k / v [b, skv, kv_h, d] with unit stride within a head, key_mask bool [b, skv] or None, out
   contiguous like q (see cdb_cross_attention).  The workspace belongs to this call."""
   b, sq, h, d = q.shape
   skv, kv_h = k.shape[1], k.shape[2]
-  qh, kh, vh = (Heads(t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)) for t in (q, k, v))
-  with torch.cuda.device(q.device):
-    need = lib().cdb_cross_attention_workspace_bytes(b, sq, skv, h, kv_h, d, int(key_mask is not None))
-    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-    st = lib().cdb_cross_attention(ctypes.byref(qh), ctypes.byref(kh), ctypes.byref(vh), _ptr(key_mask),
-                                   0 if key_mask is None else key_mask.stride(0), _ptr(out), b, sq, skv, h, kv_h, d, scale,
-                                   DTYPE_ID[q.dtype], _ptr(ws), need, _ptr(gemm_status_word(q.device)), _stream(q))
-  check(st, "cdb_cross_attention")
+  index = q.device.index
+  need = _workspace_bytes_on(index, b, sq, skv, h, kv_h, d, int(key_mask is not None))
+  ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+  qh, kh, vh = (Heads(t.data_ptr(), *t.stride()[:3]) for t in (q, k, v))
+  _on_device(index, lib().cdb_cross_attention, "cdb_cross_attention", ctypes.byref(qh), ctypes.byref(kh), ctypes.byref(vh),
+             _dp(key_mask), 0 if key_mask is None else key_mask.stride(0), out.data_ptr(), b, sq, skv, h, kv_h, d, scale,
+             DTYPE_ID[q.dtype], _dp(ws), need, _status_ptr(index))

@@ -13,7 +13,7 @@ from typing import Optional, Tuple, Union
 import torch
 
 from . import _native
-from .quantization.float4 import FORMATS, Float4Rows, empty_rows, no_gradients, one_device
+from .quantization.float4 import FORMATS, Float4Rows, empty_rows, refuse
 
 _DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 
@@ -76,33 +76,32 @@ def gated_residual_norm(x: torch.Tensor, y: Optional[torch.Tensor] = None, gate:
       raise ValueError(f"{what}: unknown 4-bit format {quantize!r}; supported: {FORMATS}")
     if dim % 32 != 0:
       raise RuntimeError(f"{what}: 4-bit rows need a width that is a multiple of 32, got {dim}")
-  tensors = dict(x=x, y=y, gate=gate, post_weight=post_weight, post_bias=post_bias, weight=weight, bias=bias, scale=scale, shift=shift)
-  one_device(what, *tensors.values())
-  no_gradients(what, *tensors.values())
+  refuse(what, x, y, gate, post_weight, post_bias, weight, bias, scale, shift)
   batch = x.shape[0] if x.dim() == 3 else 1
   x3 = _rows_of(what, "x", x, x.shape, x.dtype)
   y3 = None if y is None else _rows_of(what, "y", y, x.shape, x.dtype)
-  vectors = {name: _vector_of(what, name, tensors[name], batch, dim, x.dtype, name in ("gate", "scale", "shift"))
-             for name in ("gate", "post_weight", "post_bias", "weight", "bias", "scale", "shift")}
+  vectors = [_vector_of(what, name, t, batch, dim, x.dtype, per_batch)
+             for name, t, per_batch in (("gate", gate, True), ("post_weight", post_weight, False), ("post_bias", post_bias, False),
+                                        ("weight", weight, False), ("bias", bias, False), ("scale", scale, True), ("shift", shift, True))]
   x_out = x if y is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
-  h = None
+  h = fp4 = None
   if quantize is not None:
-    h = empty_rows(x.shape[:-1], dim, quantize, x.device)
+    h4 = empty_rows(x.shape[:-1], dim, quantize, x.device)
+    fp4 = (*h4._triple(), quantize)
     aligned = lambda t: t is None or (t.data_ptr() % 16 == 0 and all(s * t.element_size() % 16 == 0 for s in t.stride()[:-1]))
-    x3, y3 = (t if aligned(t) else t.clone(memory_format=torch.contiguous_format) for t in (x3, y3))
-    vectors = {name: t if aligned(t) else t.clone(memory_format=torch.contiguous_format) for name, t in vectors.items()}
+    x3, y3, *vectors = (t if aligned(t) else t.clone(memory_format=torch.contiguous_format) for t in (x3, y3, *vectors))
   elif norm is not None:
     h = torch.empty(x.shape, dtype=x.dtype, device=x.device)
   if x.numel():
-    _native.gated_residual_norm(x3, y3, vectors, x_out, h if quantize is None else None,
-                                None if quantize is None else (*h._triple(), quantize), post_norm, norm,
-                                float(residual_scale), float(post_eps), float(eps))
-  return x_out, h
+    _native.gated_residual_norm(x3, y3, *vectors, x_out, h, fp4, post_norm, norm, float(residual_scale), float(post_eps), float(eps))
+  return x_out, h if quantize is None else h4
 
 
 def _heads_of(t: torch.Tensor) -> torch.Tensor:
   """t [batch, tokens, heads, d] as the kernel's loads want it: unit stride within a head, every other stride positive and a
   multiple of 16 bytes, base 16-byte aligned; copied only where it is not."""
+  if t.is_contiguous() and t.data_ptr() % 16 == 0:
+    return t  # the head dimension is a multiple of 8
   ok = t.data_ptr() % 16 == 0 and (t.stride(3) == 1 or t.shape[3] == 1) and \
       all(n == 1 or (s > 0 and s % 8 == 0) for n, s in zip(t.shape[:3], t.stride()[:3]))
   return t if ok else t.clone(memory_format=torch.contiguous_format)
@@ -132,8 +131,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, key_mask:
   scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
   if not (scale > 0.0 and math.isfinite(scale)):
     raise RuntimeError(f"{what}: scale must be positive and finite, got {scale}")
-  one_device(what, q, k, v, key_mask)
-  no_gradients(what, q, k, v)
+  refuse(what, q, k, v, key_mask)
   out = torch.empty((b, sq, h, d), dtype=q.dtype, device=q.device)
   if out.numel() == 0:
     return out

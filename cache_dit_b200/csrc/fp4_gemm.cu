@@ -258,6 +258,7 @@ __global__ void __launch_bounds__(F4_THREADS, 1) fp4_gemm_kernel(const __grid_co
   if constexpr (CG == 2) cluster_sync_all();  // the peer's barriers exist before anything is signalled across the pair
   tcgen05_fence_after();
   const uint32_t tmem_base = __shfl_sync(0xffffffffu, gb->tmem_base, 0);
+  pdl_wait_prior();  // what is before this ran beside the end of the kernel that wrote the operands
 
   if (warp == 0) {
     // ---------------- TMA producer ----------------
@@ -684,18 +685,8 @@ static int f4_launch(F4Params& p, int32_t* status_word, cudaStream_t st) {
   CDB_CUDA_CHECK(attr_err);
   const int slots = CG == 2 ? sm_count() / 2 : sm_count();
   const unsigned grid = (unsigned)((p.num_tiles < slots ? p.num_tiles : slots) * CG);
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(F4_THREADS);
-  cfg.dynamicSmemBytes = (size_t)(F4_FIXED_BYTES + p.stages * p.stage_bytes);
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = CG;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = CG == 2 ? 1 : 0;
-  CDB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, fp4_gemm_kernel<CG, BN, NV, T>, p, status_word));
+  CDB_CUDA_CHECK(launch_pdl_cluster(fp4_gemm_kernel<CG, BN, NV, T>, dim3(grid), dim3(F4_THREADS),
+                                    (size_t)(F4_FIXED_BYTES + p.stages * p.stage_bytes), st, (unsigned)CG, p, status_word));
   return CDB_OK;
 }
 
@@ -807,4 +798,26 @@ extern "C" int cdb_fp4_gemm(const void* a_v, const void* w_v, const void* bias, 
               : f4_gemm<false, __nv_bfloat16>(*a, *w, bias, out, M, N, K, ld_out, gelu, status_word, st);
   return nv ? f4_gemm<true, __half>(*a, *w, bias, out, M, N, K, ld_out, gelu, status_word, st)
             : f4_gemm<false, __half>(*a, *w, bias, out, M, N, K, ld_out, gelu, status_word, st);
+}
+
+// Quantisation and product in one call: the 4-bit form of x lives in the caller's workspace.
+extern "C" size_t cdb_fp4_linear_workspace_bytes(int64_t M, int64_t K, int format) {
+  if (M <= 0 || K <= 0 || (format != CDB_NVFP4 && format != CDB_MXFP4)) return 0;
+  return (size_t)((M * (K / 2) + 255) / 256 * 256) + cdb_fp4_block_scale_bytes(M, K, format) + (size_t)M * 4;
+}
+
+extern "C" int cdb_fp4_linear(const void* x, int64_t ld_x, const void* w, const void* bias, void* out, int64_t M, int64_t N,
+                              int64_t K, int64_t ld_out, int format, int dtype, int gelu, void* workspace,
+                              size_t workspace_bytes, int32_t* status_word, void* stream) {
+  if (M == 0) return CDB_OK;
+  if (M < 0 || K <= 0 || !workspace) return CDB_ERR_BAD_ARGUMENT;
+  if (workspace_bytes < cdb_fp4_linear_workspace_bytes(M, K, format)) return CDB_ERR_SCRATCH_TOO_SMALL;
+  uint8_t* codes = static_cast<uint8_t*>(workspace);
+  uint8_t* scales = codes + (M * (K / 2) + 255) / 256 * 256;
+  const bool nv = format == CDB_NVFP4;
+  float* row = nv ? reinterpret_cast<float*>(scales + cdb_fp4_block_scale_bytes(M, K, format)) : nullptr;
+  const int rc = cdb_fp4_quant_rows(x, M, K, ld_x, dtype, format, codes, scales, row, stream);
+  if (rc != CDB_OK) return rc;
+  const F4Matrix a{codes, scales, row};
+  return cdb_fp4_gemm(&a, w, bias, out, M, N, K, ld_out, format, dtype, gelu, status_word, stream);
 }

@@ -41,7 +41,7 @@ class Float4Rows:
 
   @property
   def rows(self) -> int:
-    return self.codes.numel() * 2 // self.cols if self.cols else 0
+    return self.codes.numel() * 2 // self.cols
 
   @property
   def device(self) -> torch.device:
@@ -65,35 +65,44 @@ def _check_cols(cols: int) -> None:
     raise ValueError(f"4-bit rows need a width that is a multiple of 32 and at most {_native.FP4_MAX_COLS}, got {cols}")
 
 
-def no_gradients(what: str, *tensors) -> None:
-  """These operators have no backward pass: refuse inputs that would silently lose one."""
-  if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-    raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad() or on detached tensors")
+def refuse(what: str, *tensors) -> None:
+  """Checks every operator here makes of its tensors (None: absent): all on one CUDA device, and none that asks for a
+  gradient, which would be lost silently (no backward pass)."""
+  device = None
+  grad = torch.is_grad_enabled()
+  for t in tensors:
+    if t is None:
+      continue
+    if device is None:
+      device = t.device
+      if device.type != "cuda":
+        _native._need_cuda(t)
+    elif t.device != device:
+      _native._need_cuda(t)
+      raise RuntimeError(f"{what}: all tensors must be on one device")
+    if grad and t.requires_grad:
+      raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad() or on detached tensors")
 
 
-def one_device(what: str, *tensors) -> None:
-  present = [t for t in tensors if t is not None]
-  _native._need_cuda(*present)
-  if any(t.device != present[0].device for t in present):
-    raise RuntimeError(f"{what}: all tensors must be on one device")
-
-
-def _check_rows(t: Float4Rows, what: str) -> None:
+def _check_rows(t: Float4Rows, what: str) -> int:
+  """Refuses what is no 4-bit matrix; the number of its rows."""
+  codes, scales, row = t.codes, t.block_scales, t.row_scale
+  cols = t.cols
   _check_format(t.format)
-  _check_cols(t.cols)
-  one_device(what, *t._triple())
-  _native._need_contig(*t._triple())
-  if t.codes.dtype != torch.uint8 or t.codes.dim() < 1 or t.codes.shape[-1] * 2 != t.cols:
-    raise RuntimeError(f"{what}: codes must be uint8 [..., {t.cols // 2}], got {t.codes.dtype} {tuple(t.codes.shape)}")
-  need = _native.fp4_block_scale_bytes(t.rows, t.cols, t.format)
-  if t.block_scales.dtype != torch.uint8 or t.block_scales.numel() != need:
-    raise RuntimeError(f"{what}: block scales must be {need} bytes in tiles of 128 rows x 4 scales, got "
-                       f"{t.block_scales.dtype} {tuple(t.block_scales.shape)}")
+  _check_cols(cols)
+  if codes.dtype != torch.uint8 or codes.dim() < 1 or codes.shape[-1] * 2 != cols or not codes.is_contiguous():
+    raise RuntimeError(f"{what}: codes must be contiguous uint8 [..., {cols // 2}], got {codes.dtype} {tuple(codes.shape)}")
+  rows = codes.numel() * 2 // cols
+  need = _native.fp4_block_scale_bytes(rows, cols, t.format)
+  if scales.dtype != torch.uint8 or scales.numel() != need or not scales.is_contiguous():
+    raise RuntimeError(f"{what}: block scales must be {need} contiguous bytes in tiles of 128 rows x 4 scales, got "
+                       f"{scales.dtype} {tuple(scales.shape)}")
   if t.format == "nvfp4":
-    if t.row_scale is None or t.row_scale.dtype != torch.float32 or t.row_scale.numel() != t.rows:
-      raise RuntimeError(f"{what}: nvfp4 needs one float32 scale per row ({t.rows})")
-  elif t.row_scale is not None:
+    if row is None or row.dtype != torch.float32 or row.numel() != rows or not row.is_contiguous():
+      raise RuntimeError(f"{what}: nvfp4 needs one contiguous float32 scale per row ({rows})")
+  elif row is not None:
     raise RuntimeError(f"{what}: mxfp4 has no row scale")
+  return rows
 
 
 def empty_rows(lead, cols: int, fmt: str, device) -> Float4Rows:
@@ -106,67 +115,103 @@ def empty_rows(lead, cols: int, fmt: str, device) -> Float4Rows:
                     torch.empty(lead, dtype=torch.float32, device=device) if fmt == "nvfp4" else None, fmt, cols)
 
 
-def _as_matrix(x: torch.Tensor) -> torch.Tensor:
-  """x as [rows, cols] with unit column stride, 16-byte aligned rows; copied only where it is not."""
-  x2 = x.reshape(-1, x.shape[-1])
-  if x2.stride(-1) != 1 or (x2.shape[0] > 1 and x2.stride(0) * x2.element_size() % 16 != 0) or x2.stride(0) < x2.shape[1] \
-      or x2.data_ptr() % 16 != 0:
-    x2 = x2.clone(memory_format=torch.contiguous_format)
-  return x2
+def _as_matrix(x: torch.Tensor, rows: int, cols: int):
+  """(x as rows of `cols` elements with unit column stride and 16-byte aligned rows, their distance); copied only where it
+  is not that already."""
+  if x.is_contiguous():
+    ld = cols
+  else:
+    x = x.reshape(rows, cols)
+    ld = x.stride(0) if rows > 1 else cols
+    if x.stride(1) != 1 or ld < cols or ld * x.element_size() % 16 != 0:
+      x = x.clone(memory_format=torch.contiguous_format)
+      ld = cols
+  if x.data_ptr() % 16 != 0:
+    x = x.clone(memory_format=torch.contiguous_format)
+    ld = cols
+  return x, ld
+
+
+def _rows_to_quantise(x: torch.Tensor, dtypes, what: str):
+  if x.dtype not in dtypes or x.dim() < 1:
+    raise RuntimeError(f"{what} takes rows of {', '.join(str(d)[6:] for d in dtypes)}, got {x.dtype} {tuple(x.shape)}")
+  cols = x.shape[-1]
+  _check_cols(cols)
+  return x.numel() // cols, cols
 
 
 def float4_quantize_rows(x: torch.Tensor, format: str = "nvfp4") -> Float4Rows:
   """Quantise the rows of x [..., cols] (float32, bfloat16 or float16) to 4 bits.  An infinity or NaN makes its row
   (nvfp4) or its block of 32 (mxfp4) stand for NaN."""
+  what = "float4_quantize_rows"
   _check_format(format)
-  if x.dtype not in _DTYPES or x.dim() < 1:
-    raise RuntimeError(f"float4_quantize_rows takes rows of float32, bfloat16 or float16, got {x.dtype} {tuple(x.shape)}")
-  _check_cols(x.shape[-1])
-  one_device("float4_quantize_rows", x)
-  no_gradients("float4_quantize_rows", x)
-  out = empty_rows(x.shape[:-1], x.shape[-1], format, x.device)
-  if out.rows:
-    _native.fp4_quant_rows(_as_matrix(x), *out._triple(), format)
+  rows, cols = _rows_to_quantise(x, _DTYPES, what)
+  refuse(what, x)
+  out = empty_rows(x.shape[:-1], cols, format, x.device)
+  if rows:
+    x2, ld = _as_matrix(x, rows, cols)
+    _native.fp4_quant_rows(x2, ld, rows, cols, *out._triple(), format)
   return out
 
 
 def float4_dequantize_rows(t: Float4Rows, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
   """The values that 4-bit rows stand for, rounded once to `dtype`."""
-  _check_rows(t, "float4_dequantize_rows")
+  what = "float4_dequantize_rows"
+  rows = _check_rows(t, what)
+  refuse(what, *t._triple())
   if dtype not in _DTYPES:
-    raise RuntimeError(f"float4_dequantize_rows writes float32, bfloat16 or float16, not {dtype}")
+    raise RuntimeError(f"{what} writes float32, bfloat16 or float16, not {dtype}")
   out = torch.empty(t.shape, dtype=dtype, device=t.device)
-  if t.rows:
-    _native.fp4_dequant_rows(*t._triple(), t.cols, t.format, out.view(-1, t.cols))
+  if rows:
+    t = _aligned(t)
+    _native.fp4_dequant_rows(*t._triple(), rows, t.cols, t.format, out)
   return out
+
+
+def _aligned(t: Float4Rows) -> Float4Rows:
+  """t with 16-byte aligned codes and scales (copied only where a view starts elsewhere)."""
+  if t.codes.data_ptr() % 16 == 0 and t.block_scales.data_ptr() % 16 == 0:
+    return t
+  return dataclasses.replace(t, codes=t.codes.clone(), block_scales=t.block_scales.clone())
+
+
+def _check_weight(w: Float4Rows, bias: Optional[torch.Tensor], out_dtype: torch.dtype, what: str) -> int:
+  n = _check_rows(w, what + " (w)")
+  if w.codes.dim() != 2 or n == 0 or n % 8 != 0:
+    raise RuntimeError(f"{what}: the weight must be [N, K] with N a multiple of 8, got {tuple(w.shape)}")
+  if out_dtype not in _OUT_DTYPES:
+    raise RuntimeError(f"{what} writes bfloat16 or float16, not {out_dtype}")
+  if bias is not None and (bias.dtype != out_dtype or bias.dim() != 1 or bias.shape[0] != n or not bias.is_contiguous()):
+    raise RuntimeError(f"{what}: bias must be contiguous {out_dtype} [{n}], got {bias.dtype} {tuple(bias.shape)}")
+  return n
 
 
 def float4_scaled_mm(a: Float4Rows, w: Float4Rows, bias: Optional[torch.Tensor] = None,
                      out_dtype: torch.dtype = torch.bfloat16, gelu: bool = False) -> torch.Tensor:
   """act(a [..., K] @ w [N, K]^T + bias [N]) -> [..., N]; `gelu`: act is the tanh-GELU of the fp32 value."""
-  _check_rows(a, "float4_scaled_mm (a)")
-  _check_rows(w, "float4_scaled_mm (w)")
-  if a.format != w.format or a.cols != w.cols or w.codes.dim() != 2:
-    raise RuntimeError(f"float4_scaled_mm: operands do not match: {a.format} {tuple(a.shape)} and {w.format} {tuple(w.shape)}")
-  n = w.rows
-  if n == 0 or n % 8 != 0:
-    raise RuntimeError(f"float4_scaled_mm: the number of weight rows must be a multiple of 8, got {n}")
-  if out_dtype not in _OUT_DTYPES:
-    raise RuntimeError(f"float4_scaled_mm writes bfloat16 or float16, not {out_dtype}")
-  if bias is not None and (bias.dtype != out_dtype or tuple(bias.shape) != (n, ) or not bias.is_contiguous()):
-    raise RuntimeError(f"float4_scaled_mm: bias must be contiguous {out_dtype} [{n}]")
-  one_device("float4_scaled_mm", a.codes, w.codes, bias)
-  no_gradients("float4_scaled_mm", bias)
-  out = torch.empty((*a.shape[:-1], n), dtype=out_dtype, device=a.device)
-  if a.rows:
-    _native.fp4_gemm(a._triple(), w._triple(), bias, out.view(-1, n), a.cols, a.format, gelu)
+  what = "float4_scaled_mm"
+  rows = _check_rows(a, what + " (a)")
+  n = _check_weight(w, bias, out_dtype, what)
+  if a.format != w.format or a.cols != w.cols:
+    raise RuntimeError(f"{what}: operands do not match: {a.format} {tuple(a.shape)} and {w.format} {tuple(w.shape)}")
+  refuse(what, *a._triple(), *w._triple(), bias)
+  out = torch.empty((*a.codes.shape[:-1], n), dtype=out_dtype, device=a.device)
+  if rows:
+    _native.fp4_gemm(_aligned(a)._triple(), _aligned(w)._triple(), bias, out, rows, a.cols, a.format, gelu)
   return out
 
 
 def float4_linear(x: torch.Tensor, w: Float4Rows, bias: Optional[torch.Tensor] = None, gelu: bool = False) -> torch.Tensor:
-  """act(x @ w^T + bias) with x quantised to w's format on the way; x bfloat16 or float16, and so is the result."""
-  if x.dtype not in _OUT_DTYPES:
-    raise RuntimeError(f"float4_linear takes bfloat16 or float16 activations, got {x.dtype}")
-  if x.shape[-1] != w.cols:
-    raise RuntimeError(f"float4_linear: x has {x.shape[-1]} columns, the weight {w.cols}")
-  return float4_scaled_mm(float4_quantize_rows(x, w.format), w, bias, x.dtype, gelu)
+  """act(x @ w^T + bias) with x quantised to w's format on the way; x bfloat16 or float16, and so is the result: the same
+  numbers as float4_scaled_mm(float4_quantize_rows(x, w.format), w, bias, x.dtype, gelu)."""
+  what = "float4_linear"
+  rows, cols = _rows_to_quantise(x, _OUT_DTYPES, what)
+  n = _check_weight(w, bias, x.dtype, what)
+  if cols != w.cols:
+    raise RuntimeError(f"{what}: x has {cols} columns, the weight {w.cols}")
+  refuse(what, x, w.codes, w.block_scales, w.row_scale, bias)
+  out = torch.empty((*x.shape[:-1], n), dtype=x.dtype, device=x.device)
+  if rows:
+    x2, ld = _as_matrix(x, rows, cols)
+    _native.fp4_linear(x2, ld, _aligned(w)._triple(), bias, out, rows, cols, w.format, gelu)
+  return out

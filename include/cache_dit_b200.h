@@ -389,6 +389,12 @@ CDB_API int cdb_fp4_gemm(const void* a /* cdb_fp4_matrix */, const void* w /* cd
                          void* out, int64_t M, int64_t N, int64_t K, int64_t ld_out, int format, int dtype, int gelu,
                          int32_t* status_word, void* stream);
 
+/* cdb_fp4_quant_rows of x [M, K] (`dtype`, rows ld_x apart) and cdb_fp4_gemm in one call; the 4-bit form of x lives in
+ * `workspace` (cdb_fp4_linear_workspace_bytes(), 16-byte aligned, not zeroed, in use until the call's work is done). */
+CDB_API size_t cdb_fp4_linear_workspace_bytes(int64_t M, int64_t K, int format);
+CDB_API int cdb_fp4_linear(const void* x, int64_t ld_x, const void* w /* cdb_fp4_matrix */, const void* bias, void* out,
+                           int64_t M, int64_t N, int64_t K, int64_t ld_out, int format, int dtype, int gelu,
+                           void* workspace, size_t workspace_bytes, int32_t* status_word, void* stream);
 /* Tuning knob (no counterpart in the reference): the tile of every later 4-bit product of the process.  cols = 0: chosen
  * by size; pair = 0: one SM, 128 x cols, cols 64 or 128; pair = 1: a pair of SMs, 256 x cols, cols 128 or 256. */
 CDB_API int cdb_tuning_set_fp4_tile(int pair, int cols);
