@@ -8,15 +8,18 @@
 // One pass over the keys with a running maximum m and sum l per row (online softmax), on tensor memory:
 //   * a CTA per SM takes two tiles of 128 rows, (128 / G) queries x G heads that share a key head, so K and V are read
 //     once for the group; work items are spread over a persistent grid, K and V tiles of 128 keys come by TMA into a ring;
-//   * S = Q K^T (128 x 128 fp32) in tensor memory; a warpgroup per tile reads its row (a thread per row), writes
-//     P = exp2(S c - m c) in the tensors' type over S, and P V accumulates in tensor memory from there.  While one
-//     tile's warpgroup works on its S, the tensor core runs the other tile's products;
+//   * S = Q K^T (128 x 128 fp32) in tensor memory; a warpgroup per tile reads its row (a thread per row) and writes
+//     P = exp2(S c - m c) in the tensors' type back to tensor memory, from where P V accumulates.  P has columns of its
+//     own: as soon as S is read, the next product of scores may overwrite it, and a tile's exponentials run beside the
+//     other tile's products.  (With P over S the chain S -> P -> P V -> next S of one tile set the pace, 3600 clocks a
+//     step of both tiles; the tensor core needs 2040.)  At d > 64 there is room for one S, which the tiles take in turn;
+//   * the output goes through shared memory and TMA: stores of a thread per row took 5500 clocks a tile;
 //   * O is rescaled only when a row's maximum has grown by more than 2^8: until then P simply grows to at most 2^8, which
 //     costs nothing in a floating type.  P is rounded to 16 bits for the product (a relative 2^-9 or 2^-12 each,
 //     averaged over the keys); m, l, S and O are fp32.
 // Few rows over many keys: the key range is split over CTAs, partial (O, m, l) are joined by a second kernel.
 //
-// Warps: 0..3 and 4..7 the tiles' softmax and output, 8 TMA, 9 MMA, 10 clears masked rows of V in shared memory.
+// Warps: 0..3 and 4..7 the tiles' softmax and output, 8 TMA, 9 and 10 the tiles' products.
 // Every wait is bounded: on expiry the roles drain, tensor memory is freed and the kernel returns.
 #include <cmath>
 
@@ -25,7 +28,7 @@
 namespace cdb {
 
 constexpr int XA_THREADS = 352;
-constexpr int XA_TMA_WARP = 8, XA_MMA_WARP = 9, XA_FIX_WARP = 10;
+constexpr int XA_TMA_WARP = 8, XA_MMA_WARP = 9;  // the tiles' products: XA_MMA_WARP + t
 constexpr int XA_ROWS = 128;  // rows of a tile
 constexpr int XA_KEYS = 128;  // keys of a step
 constexpr int XA_MAX_STAGES = 10;
@@ -35,25 +38,35 @@ constexpr int XA_BOX_BYTES = 128 * 128;  // 128 rows x 64 elements
 template <int DP>
 constexpr int xa_tile_bytes() { return XA_BOX_BYTES * (DP / 64); }
 template <int DP>
-constexpr int xa_stages() { return DP == 128 ? 5 : 10; }
+constexpr int xa_stages() { return DP == 128 ? 4 : 10; }
 template <int DP>
-constexpr int xa_smem() { return 1024 + (2 + xa_stages<DP>()) * xa_tile_bytes<DP>() + 512; }
+constexpr int xa_smem() { return 1024 + (2 + xa_stages<DP>()) * xa_tile_bytes<DP>() + 2 * XA_BOX_BYTES + 512; }
+// Tensor memory columns: S (one or two) | P0 | P1 | O0 | O1.  With one S the order is P0 S P1 O0 O1.
+template <int DP>
+constexpr int xa_s_count() { return DP == 64 ? 2 : 1; }
+template <int DP>
+__host__ __device__ constexpr uint32_t xa_s_col(int t) { return DP == 64 ? 128u * (uint32_t)t : 64u; }
+template <int DP>
+__host__ __device__ constexpr uint32_t xa_p_col(int t) { return DP == 64 ? 256u + 64u * (uint32_t)t : 192u * (uint32_t)t; }
+template <int DP>
+__host__ __device__ constexpr uint32_t xa_o_col(int t) { return DP == 64 ? 384u + 64u * (uint32_t)t : 256u + 128u * (uint32_t)t; }
 static_assert(xa_smem<128>() <= 232448 && xa_smem<64>() <= 232448, "shared memory");
 
 struct __align__(8) XaBarriers {
   uint64_t q_full[2], q_empty[2];
   uint64_t kv_full[XA_MAX_STAGES], kv_empty[XA_MAX_STAGES];
-  uint64_t v_clean[XA_MAX_STAGES];  // masked rows of the stage's V are zero
-  uint64_t s_full[2];               // S in tensor memory, and with it the product before it complete
-  uint64_t p_full[2];               // P written, S and (at an item's first step) O read
-  uint64_t done[2];
+  uint64_t s_full[2];               // a tile's S is in tensor memory
+  uint64_t s_turn[2];               // S is read and a tile's products of scores may overwrite it
+  uint64_t p_full[2][2];            // P of a half of the keys written; by an item's first one its predecessor's O is read
+  uint64_t pv_done[2];              // a tile's P V complete
+  uint64_t staged[2];               // the warps of a tile meet around its output buffer
   uint32_t tmem_base;
   volatile int abort_flag;
 };
 static_assert(sizeof(XaBarriers) <= 512, "barriers");
 
 struct XaParams {
-  CUtensorMap map_q, map_k, map_v;
+  CUtensorMap map_q, map_k, map_v, map_out;
   void* out;
   float* part_o;    // [splits][rows][D], or null
   float2* part_ml;  // [splits][rows]: (m c, l)
@@ -109,6 +122,11 @@ __device__ __forceinline__ void tma_load_4d(const CUtensorMap* map, uint64_t* ba
       ::"r"(smem_u32(dst)), "l"(map), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
       : "memory");
 }
+__device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, const void* src, int c0, int c1, int c2, int c3) {
+  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(map),
+               "r"(smem_u32(src)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+               : "memory");
+}
 // tcgen05 instructions of a whole, converged warp: each elects its issuing lane itself (under a branch on an elected lane
 // the compiler spends many clocks making each operand uniform).
 #define CDB_XA_ELECTED(text) "{\n\t.reg .pred e, p;\n\telect.sync _|e, 0xffffffff;\n\t" text "\n\t}"
@@ -144,15 +162,13 @@ __device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_
         "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
-__device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_t (&r)[32]) {
+__device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
-      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
-        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]),
-        "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
-        "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
       : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -160,6 +176,54 @@ __device__ __forceinline__ float xa_exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+__device__ __forceinline__ float xa_max3(float a, float b, float c) {  // NaN if any is
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ uint64_t xa_pair(float lo, float hi) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
+  return d;
+}
+__device__ __forceinline__ void xa_unpair(uint64_t p, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(p));
+}
+__device__ __forceinline__ uint64_t xa_fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t xa_add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+// 2^x of a pair without the special-function unit, whose 16 results a clock bound the softmax: x = n + f with n the
+// nearest integer (from the low bits of x + 1.5 * 2^23), 2^f on [-1/2, 1/2] by a polynomial of degree 4 fitted for least
+// relative error (2.6e-6, far below the rounding of P), n added to the exponent.  x is held above -126: there P is nothing.
+// Every XA_POLY-th pair takes this way.
+constexpr int XA_POLY = 4;
+__device__ __forceinline__ void xa_exp2_fma(uint64_t e, float& lo, float& hi) {
+  xa_unpair(e, lo, hi);
+  lo = xa_max3(lo, -126.f, -126.f);
+  hi = xa_max3(hi, -126.f, -126.f);
+  const uint64_t x = xa_pair(lo, hi);
+  const uint64_t shifted = xa_add2(x, xa_pair(12582912.f, 12582912.f));
+  const uint64_t n = xa_add2(shifted, xa_pair(-12582912.f, -12582912.f));
+  const uint64_t f = xa_fma2(n, xa_pair(-1.f, -1.f), x);
+  uint64_t y = xa_pair(9.570102207e-3f, 9.570102207e-3f);
+  y = xa_fma2(y, f, xa_pair(5.591785908e-2f, 5.591785908e-2f));
+  y = xa_fma2(y, f, xa_pair(0.2402474433f, 0.2402474433f));
+  y = xa_fma2(y, f, xa_pair(0.6931217909f, 0.6931217909f));
+  y = xa_fma2(y, f, xa_pair(0.9999992847f, 0.9999992847f));
+  float a, b, na, nb;
+  xa_unpair(y, a, b);
+  xa_unpair(shifted, na, nb);
+  lo = __uint_as_float(__float_as_uint(a) + (__float_as_uint(na) << 23));
+  hi = __uint_as_float(__float_as_uint(b) + (__float_as_uint(nb) << 23));
 }
 template <typename T>
 __device__ __forceinline__ uint32_t xa_pack(float lo, float hi) {
@@ -182,7 +246,8 @@ __global__ void __launch_bounds__(XA_THREADS, 1) cross_attention_kernel(const __
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint8_t* s_q = smem;
   uint8_t* s_kv = smem + 2 * TILE;
-  XaBarriers* gb = reinterpret_cast<XaBarriers*>(s_kv + STAGES * TILE);
+  uint8_t* s_out = s_kv + STAGES * TILE;  // 128 rows x 64 columns of output per tile
+  XaBarriers* gb = reinterpret_cast<XaBarriers*>(s_out + 2 * XA_BOX_BYTES);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
   const int lane = threadIdx.x & 31;
   pdl_launch_dependents();
@@ -192,13 +257,15 @@ __global__ void __launch_bounds__(XA_THREADS, 1) cross_attention_kernel(const __
       mbar_init(&gb->q_full[t], 1);
       mbar_init(&gb->q_empty[t], 1);
       mbar_init(&gb->s_full[t], 1);
-      mbar_init(&gb->p_full[t], 4);
-      mbar_init(&gb->done[t], 1);
+      mbar_init(&gb->p_full[t][0], 4);
+      mbar_init(&gb->p_full[t][1], 4);
+      mbar_init(&gb->s_turn[t], 4);
+      mbar_init(&gb->pv_done[t], 1);
+      mbar_init(&gb->staged[t], 4);
     }
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(&gb->kv_full[s], 1);
-      mbar_init(&gb->kv_empty[s], 1);
-      mbar_init(&gb->v_clean[s], 1);
+      mbar_init(&gb->kv_empty[s], 2);
     }
     gb->abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -211,14 +278,13 @@ __global__ void __launch_bounds__(XA_THREADS, 1) cross_attention_kernel(const __
   __syncthreads();
   tcgen05_fence_after();
   const uint32_t tmem_base = __shfl_sync(0xffffffffu, gb->tmem_base, 0);
-  // columns: S0 | S1 | O0 | O1, 128 each; P over the first half of its S
   pdl_wait_prior();  // the mask kernel's words, and the producers of q, k, v
 
   if (warp == XA_TMA_WARP) {
     // ---------------- loads ----------------
     if (lane == 0) {
       XaRing at;
-      uint32_t issued = 0, q_uses[2] = {0, 0};
+      uint32_t issued = 0, q_uses = 0, q_used = 0;  // bit t: phase of the tile's next Q, and whether it had one
       bool ok = true;
       const uint32_t q_tx = (uint32_t)(p.g * p.q_per_tile * 128 * BOXES);
       for (int i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
@@ -228,9 +294,10 @@ __global__ void __launch_bounds__(XA_THREADS, 1) cross_attention_kernel(const __
           const int key0 = xa_key_tile(p, it, j) * XA_KEYS;
           if (j == 0) {
             for (int t = 0; t < it.tiles && ok; ++t) {
-              ok = bounded_wait(&gb->q_empty[t], (q_uses[t] & 1u) ^ 1u, &gb->abort_flag, status_word, 31);
+              ok = bounded_wait(&gb->q_empty[t], ((q_uses >> t) & 1u) ^ 1u, &gb->abort_flag, status_word, 31);
               if (!ok) break;
-              ++q_uses[t];
+              q_uses ^= 1u << t;
+              q_used |= 1u << t;
               mbar_expect_tx(&gb->q_full[t], q_tx);
               for (int x = 0; x < BOXES; ++x)
                 tma_load_4d(&p.map_q, &gb->q_full[t], s_q + t * TILE + x * XA_BOX_BYTES, x * 64, it.head0,
@@ -255,142 +322,94 @@ __global__ void __launch_bounds__(XA_THREADS, 1) cross_attention_kernel(const __
       for (uint32_t j = issued > (uint32_t)STAGES ? issued - STAGES : 0; j < issued; ++j)
         while (!mbar_try_wait(&gb->kv_full[j % STAGES], (j / STAGES) & 1u) && global_timer_ns() - t0 < BARRIER_LIMIT_NS) {}
       for (int t = 0; t < 2; ++t)
-        while (q_uses[t] != 0 && !mbar_try_wait(&gb->q_full[t], (q_uses[t] - 1) & 1u) && global_timer_ns() - t0 < BARRIER_LIMIT_NS) {}
+        while (((q_used >> t) & 1u) && !mbar_try_wait(&gb->q_full[t], ((q_uses >> t) & 1u) ^ 1u) && global_timer_ns() - t0 < BARRIER_LIMIT_NS) {}
     }
     __syncwarp();
-  } else if (warp == XA_MMA_WARP) {
-    // ---------------- products: O_t += P_t V(step), then S_t = Q_t K(next step)^T, for both tiles in turn ----------------
+  } else if (warp >= XA_MMA_WARP) {
+    // ---------------- products of tile t ----------------
+    // For every step: S = Q_t K^T, then O_t += P_t V of the step before, whose exponentials ran meanwhile.  A warp per
+    // tile: a satisfied wait takes a hundred clocks, and one warp that did them all for both tiles set the pace.
+    const int t = warp - XA_MMA_WARP;
     constexpr uint32_t idesc_s = xa_idesc(BF16, XA_KEYS, false);
     constexpr uint32_t idesc_o = xa_idesc(BF16, DP, true);
-    const uint32_t q_base = __shfl_sync(0xffffffffu, smem_u32(s_q), 0);
-    const uint32_t kv_base = __shfl_sync(0xffffffffu, smem_u32(s_kv), 0);
+    const uint32_t q_base = smem_u32(s_q) + t * TILE;
+    const uint32_t kv_base = smem_u32(s_kv);
+    const uint32_t s_addr = tmem_base + (t ? xa_s_col<DP>(1) : xa_s_col<DP>(0));
+    const uint32_t p_addr = tmem_base + (t ? xa_p_col<DP>(1) : xa_p_col<DP>(0));
+    const uint32_t o_addr = tmem_base + (t ? xa_o_col<DP>(1) : xa_o_col<DP>(0));
     auto wait = [&](uint64_t* bar, uint32_t phase, int code) {
       return __all_sync(0xffffffffu, bounded_wait(bar, phase, &gb->abort_flag, status_word, code)) != 0;
     };
-    auto scores = [&](int t, int stage) {
-      const uint64_t a = make_kmajor_sw128_desc(q_base + t * TILE), b = make_kmajor_sw128_desc(kv_base + stage * TILE);
-#pragma unroll
-      for (int k = 0; k < DP / 16; ++k) {  // 16 elements = 32 bytes; a box holds 64
-        const uint64_t off = (uint64_t)((k / 4) * (XA_BOX_BYTES >> 4) + (k % 4) * 2);
-        xa_mma_ss(tmem_base + t * 128, a + off, b + off, idesc_s, k != 0);
-      }
-      xa_commit(&gb->s_full[t]);
-    };
-    XaRing at;  // the next K or V tile in the ring
-    uint32_t p_uses[2] = {0, 0}, q_uses[2] = {0, 0};
+    bool due = false, due_first = false;  // a P V to be issued
+    int due_stage = 0;
+    uint32_t due_phase = 0;
+    XaRing at;  // K of the current step; V follows it
+    uint32_t p_uses = 0, q_uses = 0, turns = 0;
     bool ok = true;
-    int i = blockIdx.x, j = 0;
-    XaItem cur{};
-    auto find = [&](int& i, XaItem& it) {  // the first item from i on with work
-      for (; i < p.items; i += gridDim.x) {
-        it = xa_item(p, i);
-        if (it.steps > 0) return true;
-      }
-      return false;
-    };
-    bool have = find(i, cur);
-    if (have) {
-      ok = wait(&gb->kv_full[at.stage], at.phase, 33);
-      for (int t = 0; t < cur.tiles && ok; ++t) {
-        ok = wait(&gb->q_full[t], q_uses[t] & 1u, 34);
-        if (!ok) break;
-        ++q_uses[t];
+    auto values = [&] {  // O_t += P_t V
+      ok = wait(&gb->kv_full[due_stage], due_phase, 35);
+      const uint64_t v = xa_v_desc(kv_base + due_stage * TILE);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        if (ok) ok = wait(&gb->p_full[t][half], p_uses & 1u, 36);
+        if (!ok) return;
         tcgen05_fence_after();
-        scores(t, at.stage);
-        if (cur.steps == 1) xa_commit(&gb->q_empty[t]);
-      }
-      if (ok) xa_commit(&gb->kv_empty[at.stage]);
-      at.next(STAGES);
-    }
-    while (have && ok) {
-      int ni = i, nj = j + 1;
-      XaItem next = cur;
-      bool more = true;
-      if (nj == cur.steps) {
-        nj = 0;
-        ni = i + gridDim.x;
-        more = find(ni, next);
-      }
-      const int v_stage = at.stage;
-      ok = wait(&gb->kv_full[v_stage], at.phase, 35);
-      if (ok && p.words != nullptr) ok = wait(&gb->v_clean[v_stage], at.phase, 36);
-      if (!ok) break;
-      at.next(STAGES);
-      const uint64_t v = xa_v_desc(kv_base + v_stage * TILE);
-      bool k_ready = false;
-      for (int t = 0; t < 2 && ok; ++t) {
-        if (t < cur.tiles) {
-          ok = wait(&gb->p_full[t], p_uses[t] & 1u, 37);
-          if (!ok) break;
-          ++p_uses[t];
-          tcgen05_fence_after();
 #pragma unroll
-          for (int k = 0; k < XA_KEYS / 16; ++k)  // 16 keys: 8 columns of P, 2048 bytes of V
-            xa_mma_ts(tmem_base + 256 + t * 128, tmem_base + t * 128 + k * 8, v + (uint64_t)(k * (2048 >> 4)), idesc_o, (j | k) != 0);
-        }
-        if (t == (cur.tiles - 1)) xa_commit(&gb->kv_empty[v_stage]);
-        if (more && t < next.tiles) {
-          if (!k_ready) {
-            ok = wait(&gb->kv_full[at.stage], at.phase, 38);
-            if (!ok) break;
-            k_ready = true;
-          }
-          if (nj == 0) {
-            ok = wait(&gb->q_full[t], q_uses[t] & 1u, 39);
-            if (!ok) break;
-            ++q_uses[t];
-          }
-          tcgen05_fence_after();
-          scores(t, at.stage);
-          if (nj + 1 == next.steps) xa_commit(&gb->q_empty[t]);
-        }
+        for (int k = half * 4; k < half * 4 + 4; ++k)  // 16 keys: 8 columns of P, 2048 bytes of V
+          xa_mma_ts(o_addr, p_addr + k * 8, v + (uint64_t)(k * (2048 >> 4)), idesc_o, !due_first || k != 0);
       }
-      if (!ok) break;
-      if (more) {
-        xa_commit(&gb->kv_empty[at.stage]);
+      xa_commit(&gb->pv_done[t]);
+      xa_commit(&gb->kv_empty[due_stage]);
+      ++p_uses;
+      due = false;
+    };
+    // After the last item one more round without scores: it issues what is outstanding.
+    for (int i = blockIdx.x; ok && (i < p.items || due); i += gridDim.x) {
+      XaItem it{};
+      if (i < p.items) it = xa_item(p, i);
+      if (i >= p.items || (t >= it.tiles && it.steps > 0)) {
+        if (due) values();
+        if (!ok) break;
+      }
+      for (int j = 0; j < it.steps && ok; ++j) {
+        const int k_stage = at.stage;
+        ok = wait(&gb->kv_full[k_stage], at.phase, 33);
+        if (!ok) break;
         at.next(STAGES);
-      }
-      have = more;
-      i = ni;
-      j = nj;
-      cur = next;
-    }
-    if (ok) {
-      xa_commit(&gb->done[0]);
-      xa_commit(&gb->done[1]);
-    }
-    __syncwarp();
-  } else if (warp == XA_FIX_WARP) {
-    // ---------------- rows of V that the mask leaves out become zero: 0 * NaN would not be 0 ----------------
-    if (p.words != nullptr) {
-      XaRing at;
-      bool ok = true;
-      for (int i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
-        const XaItem it = xa_item(p, i);
-        for (int j = 0; j < it.steps; ++j) {
-          const uint4 w = __ldg(reinterpret_cast<const uint4*>(p.words) + (int64_t)it.b * p.key_tiles + xa_key_tile(p, it, j));
-          const uint32_t word[4] = {w.x, w.y, w.z, w.w};
-          for (int kv = 0; kv < 2; ++kv) {  // K passes through untouched: a stage's barrier turns over with every use
-            ok = __all_sync(0xffffffffu, bounded_wait(&gb->kv_full[at.stage], at.phase, &gb->abort_flag, status_word, 40));
-            if (!ok) break;
-            if (kv == 1 && (w.x & w.y & w.z & w.w) != 0xffffffffu) {
-              uint8_t* tile = s_kv + at.stage * TILE;
-#pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                for (uint32_t left = ~word[q]; left != 0; left &= left - 1) {  // a row is 128 bytes in each box
-                  const int r = q * 32 + __ffs(left) - 1;
-#pragma unroll
-                  for (int x = 0; x < BOXES; ++x) *reinterpret_cast<uint32_t*>(tile + x * XA_BOX_BYTES + r * 128 + lane * 4) = 0u;
-                }
-              }
-              fence_async_smem();
-            }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&gb->v_clean[at.stage]);
-            at.next(STAGES);
-          }
+        if (t >= it.tiles) {  // the other tile's alone: K and V are released for this one
+          if (lane == 0) mbar_arrive(&gb->kv_empty[k_stage]);
+          ok = wait(&gb->kv_full[at.stage], at.phase, 38);
           if (!ok) break;
+          if (lane == 0) mbar_arrive(&gb->kv_empty[at.stage]);
+          at.next(STAGES);
+          continue;
         }
+        if (j == 0) {
+          ok = wait(&gb->q_full[t], q_uses & 1u, 34);
+          if (!ok) break;
+          ++q_uses;
+        }
+        // Two S: this tile's last one is read.  One S: the tiles take turns, and who read the last one passes the turn on;
+        // so every phase of a turn belongs to one product.  The first product of all finds S free.
+        ok = wait(&gb->s_turn[t], (turns & 1u) ^ (DP == 64 || t == 0 ? 1u : 0u), 37);
+        if (!ok) break;
+        ++turns;
+        tcgen05_fence_after();
+        const uint64_t a = make_kmajor_sw128_desc(q_base), b = make_kmajor_sw128_desc(kv_base + k_stage * TILE);
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k) {  // 16 elements = 32 bytes; a box holds 64
+          const uint64_t off = (uint64_t)((k / 4) * (XA_BOX_BYTES >> 4) + (k % 4) * 2);
+          xa_mma_ss(s_addr, a + off, b + off, idesc_s, k != 0);
+        }
+        xa_commit(&gb->s_full[t]);
+        if (j + 1 == it.steps) xa_commit(&gb->q_empty[t]);
+        xa_commit(&gb->kv_empty[k_stage]);
+        if (due) values();
+        due = true;
+        due_first = j == 0;
+        due_stage = at.stage;
+        due_phase = at.phase;
+        at.next(STAGES);
       }
     }
     __syncwarp();
@@ -399,45 +418,76 @@ __global__ void __launch_bounds__(XA_THREADS, 1) cross_attention_kernel(const __
     const int t = warp >> 2;
     const int row = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t s_addr = tmem_base + lanes + t * 128;
-    const uint32_t o_addr = tmem_base + lanes + 256 + t * 128;
+    const uint32_t s_addr = tmem_base + lanes + (t ? xa_s_col<DP>(1) : xa_s_col<DP>(0));
+    const uint32_t p_addr = tmem_base + lanes + (t ? xa_p_col<DP>(1) : xa_p_col<DP>(0));
+    const uint32_t o_addr = tmem_base + lanes + (t ? xa_o_col<DP>(1) : xa_o_col<DP>(0));
+    XaRing at;  // follows the ring of K and V tiles where there is a mask
     uint32_t s_uses = 0;
     bool ok = true;
-    // What the last item's output needs, written when the next one's first S is there (its O is complete then).
+    // What the last item's output needs; it is written once its last P V is complete, while the next one's scores wait.
     bool pending = false;
+    int out_b = 0, out_q0 = 0, out_head0 = 0;
     int64_t out_row = -1;   // row of `out`, -1: none (beyond the last query, or a row of no head)
     int64_t part_base = 0;  // first row of the split's partial results
     float m = 0.f, l = 0.f;
+    uint32_t meetings = 0;
+    auto meet = [&] {  // the tile's four warps; bounded like every wait here
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&gb->staged[t]);
+      return __all_sync(0xffffffffu, bounded_wait(&gb->staged[t], meetings++ & 1u, &gb->abort_flag, status_word, 43)) != 0;
+    };
     auto write_out = [&] {
+      pending = false;
       const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // NaN stays
+      if (p.part_o != nullptr) {
+        float* dst = p.part_o + (part_base + out_row) * p.d;
 #pragma unroll 1
-      for (int c0 = 0; c0 < DP; c0 += 32) {
-        if (c0 >= p.d) break;
-        uint32_t o[32];
-        tmem_ld_32x32b_x32(o_addr + c0, o);
-        tmem_ld_wait();
-        if (out_row < 0) continue;
-        if (p.part_o != nullptr) {
-          float* dst = p.part_o + (part_base + out_row) * p.d + c0;
+        for (int c0 = 0; c0 < DP && c0 < p.d; c0 += 16) {
+          uint32_t o[16];
+          tmem_ld_32x32b_x16(o_addr + c0, o);
+          tmem_ld_wait();
+          if (out_row < 0) continue;
 #pragma unroll
-          for (int x = 0; x < 8; ++x)
-            if (c0 + 4 * x < p.d) *reinterpret_cast<uint4*>(dst + 4 * x) = make_uint4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
-        } else {
-          T* dst = static_cast<T*>(p.out) + out_row * p.d + c0;
+          for (int x = 0; x < 4; ++x)
+            if (c0 + 4 * x < p.d) *reinterpret_cast<uint4*>(dst + c0 + 4 * x) = make_uint4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
+        }
+        if (out_row >= 0) p.part_ml[part_base + out_row] = make_float2(m == NEG_INF ? 0.f : m * p.c, l);
+      } else {
+        // 64 columns at a time through shared memory (128-byte rows, swizzled as the tensor map has it); the copy out clips
+        // queries and columns that do not exist
+        uint8_t* box = s_out + t * XA_BOX_BYTES;
+#pragma unroll 1
+        for (int x = 0; x < BOXES; ++x) {
+          if (threadIdx.x % 128 == 0) bulk_wait_group_read<0>();  // the copy before this one has read the buffer
+          if (!meet()) return false;
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            if (c0 + 8 * x < p.d) {
+          for (int h = 0; h < 4; ++h) {
+            uint32_t o[16];
+            tmem_ld_32x32b_x16(o_addr + x * 64 + h * 16, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
               uint32_t w[4];
 #pragma unroll
-              for (int y = 0; y < 4; ++y)
-                w[y] = xa_pack<T>(__uint_as_float(o[8 * x + 2 * y]) * inv, __uint_as_float(o[8 * x + 2 * y + 1]) * inv);
-              *reinterpret_cast<uint4*>(dst + 8 * x) = make_uint4(w[0], w[1], w[2], w[3]);
+              for (int z = 0; z < 4; ++z)
+                w[z] = xa_pack<T>(__uint_as_float(o[8 * y + 2 * z]) * inv, __uint_as_float(o[8 * y + 2 * z + 1]) * inv);
+              *reinterpret_cast<uint4*>(box + row * 128 + (((h * 2 + y) ^ (row & 7)) * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
             }
+          }
+          fence_async_smem();
+          if (!meet()) return false;
+          if (threadIdx.x % 128 == 0) {
+            tma_store_4d(&p.map_out, box, x * 64, out_head0, out_q0, out_b);
+            bulk_commit_group();
           }
         }
       }
-      if (out_row >= 0 && p.part_o != nullptr) p.part_ml[part_base + out_row] = make_float2(m == NEG_INF ? 0.f : m * p.c, l);
-      pending = false;
+      return true;
+    };
+    uint32_t posted = 0;
+    // The tile's last P V is complete: its P may be overwritten, its O read.
+    auto values_done = [&] {
+      return posted == 0 || __all_sync(0xffffffffu, bounded_wait(&gb->pv_done[t], (posted - 1) & 1u, &gb->abort_flag, status_word, 42)) != 0;
     };
     for (int i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
       const XaItem it = xa_item(p, i);
@@ -445,7 +495,10 @@ __global__ void __launch_bounds__(XA_THREADS, 1) cross_attention_kernel(const __
       const int s = it.q0 + t * p.q_per_tile + qi;
       const int64_t next_row = qi < p.q_per_tile && s < p.sq ? ((int64_t)it.b * p.sq + s) * p.heads + it.head0 + h : -1;
       const int64_t next_base = (int64_t)it.split * p.batch * p.sq * p.heads;
-      if (t >= it.tiles) continue;
+      if (t >= it.tiles) {
+        for (int j = 0; j < 2 * it.steps; ++j) at.next(STAGES);
+        continue;
+      }
       if (it.steps == 0) {  // no key is kept: zeros (or an empty part)
         if (next_row >= 0) {
           if (p.part_o != nullptr) {
@@ -471,77 +524,119 @@ __global__ void __launch_bounds__(XA_THREADS, 1) cross_attention_kernel(const __
         if (!ok) break;
         ++s_uses;
         tcgen05_fence_after();
-        if (pending) write_out();
-        float v[4][32];
+        uint32_t v[4][32];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) tmem_ld_32x32b_x32(s_addr + q * 32, reinterpret_cast<uint32_t(&)[32]>(v[q]));
+        for (int q = 0; q < 4; ++q) tmem_ld_32x32b_x32(s_addr + q * 32, v[q]);
+        if (p.words != nullptr) {
+          // Rows of V that the mask leaves out become zero: 0 * NaN would not be 0.  A thread of tile 0 per key; the
+          // products wait for this tile's P before they read V for either.
+          at.next(STAGES);  // K
+          if (t == 0 && (w.x & w.y & w.z & w.w) != 0xffffffffu) {
+            ok = __all_sync(0xffffffffu, bounded_wait(&gb->kv_full[at.stage], at.phase, &gb->abort_flag, status_word, 40));
+            if (!ok) break;
+            const uint32_t word = (warp & 2) ? ((warp & 1) ? w.w : w.z) : ((warp & 1) ? w.y : w.x);
+            if (!((word >> lane) & 1u)) {
+              uint4* v_row = reinterpret_cast<uint4*>(s_kv + at.stage * TILE + row * 128);  // 128 bytes in each box
+#pragma unroll
+              for (int x = 0; x < BOXES; ++x)
+#pragma unroll
+                for (int y = 0; y < 8; ++y) v_row[x * (XA_BOX_BYTES / 16) + y] = make_uint4(0, 0, 0, 0);
+            }
+            fence_async_smem();
+          }
+          at.next(STAGES);  // V
+        }
         tmem_ld_wait();
+        tcgen05_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&gb->s_turn[DP == 64 ? t : (t == 0 && it.tiles == 2 ? 1 : 0)]);  // the next scores may overwrite S
         if ((w.x & w.y & w.z & w.w) != 0xffffffffu) {
           const uint32_t word[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
           for (int q = 0; q < 4; ++q)
 #pragma unroll
-            for (int x = 0; x < 32; ++x) v[q][x] = (word[q] >> x) & 1u ? v[q][x] : NEG_INF;
+            for (int x = 0; x < 32; ++x) v[q][x] = (word[q] >> x) & 1u ? v[q][x] : 0xff800000u;
         }
         float top4[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          top4[q] = v[q][0];
+          top4[q] = xa_max3(__uint_as_float(v[q][0]), __uint_as_float(v[q][1]), __uint_as_float(v[q][2]));
 #pragma unroll
-          for (int x = 1; x < 32; ++x) top4[q] = fmaxf(top4[q], v[q][x]);
+          for (int x = 3; x < 31; x += 2) top4[q] = xa_max3(top4[q], __uint_as_float(v[q][x]), __uint_as_float(v[q][x + 1]));
+          top4[q] = xa_max3(top4[q], top4[q], __uint_as_float(v[q][31]));
         }
-        const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3]));
+        const float top = xa_max3(xa_max3(top4[0], top4[1], top4[2]), top4[3], top4[3]);
+        ok = values_done();
+        if (!ok) break;
+        tcgen05_fence_after();
+        if (pending) ok = write_out();
+        if (!ok) break;
         if (j == 0) {
           m = top;
           l = 0.f;
-        } else if (__any_sync(0xffffffffu, (top - m) * p.c > XA_LAZY || (m == NEG_INF && top > NEG_INF))) {
-          const float grown = fmaxf(m, top);
+        } else if (__any_sync(0xffffffffu, !((top - m) * p.c <= XA_LAZY))) {  // a NaN too
+          const float grown = xa_max3(m, top, top);
           const float f = m == NEG_INF ? 0.f : xa_exp2((m - grown) * p.c);
           m = grown;
           l *= f;
 #pragma unroll 1
-          for (int c0 = 0; c0 < DP; c0 += 32) {
-            uint32_t o[32];
-            tmem_ld_32x32b_x32(o_addr + c0, o);
+          for (int c0 = 0; c0 < DP; c0 += 16) {
+            uint32_t o[16];
+            tmem_ld_32x32b_x16(o_addr + c0, o);
             tmem_ld_wait();
 #pragma unroll
-            for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
-            tmem_st_32x32b_x32(o_addr + c0, o);
+            for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
+            tmem_st_32x32b_x16(o_addr + c0, o);
           }
           tmem_st_wait();
         }
-        const float mc = m == NEG_INF ? 0.f : m * p.c;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        // A row of -inf alone has P = 0; one with an infinity becomes NaN whichever way its exponentials are computed.
+        const float mc = m == NEG_INF ? 0.f : m == INFINITY ? NAN : m * p.c;
+        const uint64_t c2 = xa_pair(p.c, p.c), mc2 = xa_pair(-mc, -mc);
+        uint64_t sum2[2] = {0, 0};
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           uint32_t pk[16];
 #pragma unroll
-          for (int x = 0; x < 32; ++x) {
-            v[q][x] = xa_exp2(fmaf(v[q][x], p.c, -mc));
-            sum[x & 3] += v[q][x];
+          for (int x = 0; x < 16; ++x) {
+            uint64_t e = xa_fma2(xa_pair(__uint_as_float(v[q][2 * x]), __uint_as_float(v[q][2 * x + 1])), c2, mc2);
+            float lo, hi;
+            if (x % XA_POLY == XA_POLY - 1) {
+              xa_exp2_fma(e, lo, hi);
+            } else {
+              xa_unpair(e, lo, hi);
+              lo = xa_exp2(lo);
+              hi = xa_exp2(hi);
+            }
+            sum2[x & 1] = xa_add2(sum2[x & 1], xa_pair(lo, hi));
+            pk[x] = xa_pack<T>(lo, hi);
           }
-#pragma unroll
-          for (int x = 0; x < 16; ++x) pk[x] = xa_pack<T>(v[q][2 * x], v[q][2 * x + 1]);
-          tmem_st_32x32b_x16(s_addr + q * 16, pk);
+          tmem_st_32x32b_x16(p_addr + q * 16, pk);
+          if (q & 1) {  // the products over these 64 keys may start
+            tmem_st_wait();
+            tcgen05_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&gb->p_full[t][q >> 1]);
+          }
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        tmem_st_wait();
-        tcgen05_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&gb->p_full[t]);
+        float l0, l1;
+        xa_unpair(xa_add2(sum2[0], sum2[1]), l0, l1);
+        l += l0 + l1;
+        ++posted;
       }
       if (!ok) break;
       pending = true;
       out_row = next_row;
       part_base = next_base;
+      out_b = it.b;
+      out_q0 = it.q0 + t * p.q_per_tile;
+      out_head0 = it.head0;
     }
-    if (ok && pending) {
-      ok = __all_sync(0xffffffffu, bounded_wait(&gb->done[t], 0, &gb->abort_flag, status_word, 42));
-      if (ok) {
-        tcgen05_fence_after();
-        write_out();
-      }
+    if (ok && pending && values_done()) {
+      tcgen05_fence_after();
+      write_out();
     }
+    if (threadIdx.x % 128 == 0) bulk_wait_group_all();  // the output is written before the CTA retires
     __syncwarp();
   }
 
@@ -761,6 +856,7 @@ extern "C" int cdb_cross_attention(const void* q_v, const void* k_v, const void*
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   XaParams p{};
   if (!xa_map(&p.map_q, bf16, *q, d, heads, sq, batch, plan.g, plan.q_per_tile) ||
+      !xa_map(&p.map_out, bf16, cdb_heads{out, sq * heads * d, heads * d, d}, d, heads, sq, batch, plan.g, plan.q_per_tile) ||
       !xa_map(&p.map_k, bf16, *k, d, kv_heads, skv, batch, 1, XA_KEYS) || !xa_map(&p.map_v, bf16, *v, d, kv_heads, skv, batch, 1, XA_KEYS)) {
     set_cuda_error(cudaErrorUnknown, "cuTensorMapEncodeTiled");
     return CDB_ERR_CUDA;
