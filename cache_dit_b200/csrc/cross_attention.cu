@@ -33,8 +33,10 @@ constexpr int XA_ROWS = 128;  // rows of a tile
 constexpr int XA_KEYS = 128;  // keys of a step
 constexpr int XA_MAX_STAGES = 10;
 constexpr int XA_MAX_SPLIT = 64;
+constexpr int XA_MAX_GROUP = 32;  // heads of a tile
 constexpr float XA_LAZY = 8.0f;  // log2 of how far P may grow before O is rescaled
 constexpr int XA_BOX_BYTES = 128 * 128;  // 128 rows x 64 elements
+constexpr int XA_WARP_BOX = XA_BOX_BYTES / 4;
 template <int DP>
 constexpr int xa_tile_bytes() { return XA_BOX_BYTES * (DP / 64); }
 template <int DP>
@@ -59,7 +61,6 @@ struct __align__(8) XaBarriers {
   uint64_t s_turn[2];               // S is read and a tile's products of scores may overwrite it
   uint64_t p_full[2][2];            // P of a half of the keys written; by an item's first one its predecessor's O is read
   uint64_t pv_done[2];              // a tile's P V complete
-  uint64_t staged[2];               // the warps of a tile meet around its output buffer
   uint32_t tmem_base;
   volatile int abort_flag;
 };
@@ -201,30 +202,6 @@ __device__ __forceinline__ uint64_t xa_add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
-// 2^x of a pair without the special-function unit, whose 16 results a clock bound the softmax: x = n + f with n the
-// nearest integer (from the low bits of x + 1.5 * 2^23), 2^f on [-1/2, 1/2] by a polynomial of degree 4 fitted for least
-// relative error (2.6e-6, far below the rounding of P), n added to the exponent.  x is held above -126: there P is nothing.
-// Every XA_POLY-th pair takes this way.
-constexpr int XA_POLY = 4;
-__device__ __forceinline__ void xa_exp2_fma(uint64_t e, float& lo, float& hi) {
-  xa_unpair(e, lo, hi);
-  lo = xa_max3(lo, -126.f, -126.f);
-  hi = xa_max3(hi, -126.f, -126.f);
-  const uint64_t x = xa_pair(lo, hi);
-  const uint64_t shifted = xa_add2(x, xa_pair(12582912.f, 12582912.f));
-  const uint64_t n = xa_add2(shifted, xa_pair(-12582912.f, -12582912.f));
-  const uint64_t f = xa_fma2(n, xa_pair(-1.f, -1.f), x);
-  uint64_t y = xa_pair(9.570102207e-3f, 9.570102207e-3f);
-  y = xa_fma2(y, f, xa_pair(5.591785908e-2f, 5.591785908e-2f));
-  y = xa_fma2(y, f, xa_pair(0.2402474433f, 0.2402474433f));
-  y = xa_fma2(y, f, xa_pair(0.6931217909f, 0.6931217909f));
-  y = xa_fma2(y, f, xa_pair(0.9999992847f, 0.9999992847f));
-  float a, b, na, nb;
-  xa_unpair(y, a, b);
-  xa_unpair(shifted, na, nb);
-  lo = __uint_as_float(__float_as_uint(a) + (__float_as_uint(na) << 23));
-  hi = __uint_as_float(__float_as_uint(b) + (__float_as_uint(nb) << 23));
-}
 template <typename T>
 __device__ __forceinline__ uint32_t xa_pack(float lo, float hi) {
   if constexpr (__is_same(T, __nv_bfloat16)) {
@@ -246,7 +223,7 @@ __global__ void __launch_bounds__(XA_THREADS, 1) cross_attention_kernel(const __
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint8_t* s_q = smem;
   uint8_t* s_kv = smem + 2 * TILE;
-  uint8_t* s_out = s_kv + STAGES * TILE;  // 128 rows x 64 columns of output per tile
+  uint8_t* s_out = s_kv + STAGES * TILE;  // 32 rows x 64 columns of output per softmax warp
   XaBarriers* gb = reinterpret_cast<XaBarriers*>(s_out + 2 * XA_BOX_BYTES);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
   const int lane = threadIdx.x & 31;
@@ -261,7 +238,6 @@ __global__ void __launch_bounds__(XA_THREADS, 1) cross_attention_kernel(const __
       mbar_init(&gb->p_full[t][1], 4);
       mbar_init(&gb->s_turn[t], 4);
       mbar_init(&gb->pv_done[t], 1);
-      mbar_init(&gb->staged[t], 4);
     }
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(&gb->kv_full[s], 1);
@@ -338,7 +314,7 @@ __global__ void __launch_bounds__(XA_THREADS, 1) cross_attention_kernel(const __
     const uint32_t p_addr = tmem_base + (t ? xa_p_col<DP>(1) : xa_p_col<DP>(0));
     const uint32_t o_addr = tmem_base + (t ? xa_o_col<DP>(1) : xa_o_col<DP>(0));
     auto wait = [&](uint64_t* bar, uint32_t phase, int code) {
-      return __all_sync(0xffffffffu, bounded_wait(bar, phase, &gb->abort_flag, status_word, code)) != 0;
+      return warp_wait(bar, phase, &gb->abort_flag, status_word, code);
     };
     bool due = false, due_first = false;  // a P V to be issued
     int due_stage = 0;
@@ -430,12 +406,6 @@ __global__ void __launch_bounds__(XA_THREADS, 1) cross_attention_kernel(const __
     int64_t out_row = -1;   // row of `out`, -1: none (beyond the last query, or a row of no head)
     int64_t part_base = 0;  // first row of the split's partial results
     float m = 0.f, l = 0.f;
-    uint32_t meetings = 0;
-    auto meet = [&] {  // the tile's four warps; bounded like every wait here
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&gb->staged[t]);
-      return __all_sync(0xffffffffu, bounded_wait(&gb->staged[t], meetings++ & 1u, &gb->abort_flag, status_word, 43)) != 0;
-    };
     auto write_out = [&] {
       pending = false;
       const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // NaN stays
@@ -453,13 +423,13 @@ __global__ void __launch_bounds__(XA_THREADS, 1) cross_attention_kernel(const __
         }
         if (out_row >= 0) p.part_ml[part_base + out_row] = make_float2(m == NEG_INF ? 0.f : m * p.c, l);
       } else {
-        // 64 columns at a time through shared memory (128-byte rows, swizzled as the tensor map has it); the copy out clips
-        // queries and columns that do not exist
-        uint8_t* box = s_out + t * XA_BOX_BYTES;
+        // This warp's 32 rows, 64 columns at a time, through shared memory (128-byte rows, swizzled as the tensor map has
+        // it); the copy out clips queries and columns that do not exist.
+        uint8_t* box = s_out + warp * XA_WARP_BOX;
 #pragma unroll 1
         for (int x = 0; x < BOXES; ++x) {
-          if (threadIdx.x % 128 == 0) bulk_wait_group_read<0>();  // the copy before this one has read the buffer
-          if (!meet()) return false;
+          if (lane == 0) bulk_wait_group_read<0>();  // the copy before this one has read the buffer
+          __syncwarp();
 #pragma unroll
           for (int h = 0; h < 4; ++h) {
             uint32_t o[16];
@@ -471,23 +441,22 @@ __global__ void __launch_bounds__(XA_THREADS, 1) cross_attention_kernel(const __
 #pragma unroll
               for (int z = 0; z < 4; ++z)
                 w[z] = xa_pack<T>(__uint_as_float(o[8 * y + 2 * z]) * inv, __uint_as_float(o[8 * y + 2 * z + 1]) * inv);
-              *reinterpret_cast<uint4*>(box + row * 128 + (((h * 2 + y) ^ (row & 7)) * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
+              *reinterpret_cast<uint4*>(box + lane * 128 + (((h * 2 + y) ^ (lane & 7)) * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
             }
           }
           fence_async_smem();
-          if (!meet()) return false;
-          if (threadIdx.x % 128 == 0) {
-            tma_store_4d(&p.map_out, box, x * 64, out_head0, out_q0, out_b);
+          __syncwarp();
+          if (lane == 0) {
+            if (out_q0 < p.sq) tma_store_4d(&p.map_out, box, x * 64, out_head0, out_q0, out_b);
             bulk_commit_group();
           }
         }
       }
-      return true;
     };
     uint32_t posted = 0;
     // The tile's last P V is complete: its P may be overwritten, its O read.
     auto values_done = [&] {
-      return posted == 0 || __all_sync(0xffffffffu, bounded_wait(&gb->pv_done[t], (posted - 1) & 1u, &gb->abort_flag, status_word, 42)) != 0;
+      return posted == 0 || warp_wait(&gb->pv_done[t], (posted - 1) & 1u, &gb->abort_flag, status_word, 42);
     };
     for (int i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
       const XaItem it = xa_item(p, i);
@@ -520,7 +489,7 @@ __global__ void __launch_bounds__(XA_THREADS, 1) cross_attention_kernel(const __
           auto bits = [](int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u; };
           w = make_uint4(bits(left), bits(left - 32), bits(left - 64), bits(left - 96));
         }
-        ok = __all_sync(0xffffffffu, bounded_wait(&gb->s_full[t], s_uses & 1u, &gb->abort_flag, status_word, 41));
+        ok = warp_wait(&gb->s_full[t], s_uses & 1u, &gb->abort_flag, status_word, 41);
         if (!ok) break;
         ++s_uses;
         tcgen05_fence_after();
@@ -528,11 +497,11 @@ __global__ void __launch_bounds__(XA_THREADS, 1) cross_attention_kernel(const __
 #pragma unroll
         for (int q = 0; q < 4; ++q) tmem_ld_32x32b_x32(s_addr + q * 32, v[q]);
         if (p.words != nullptr) {
-          // Rows of V that the mask leaves out become zero: 0 * NaN would not be 0.  A thread of tile 0 per key; the
-          // products wait for this tile's P before they read V for either.
+          // Rows of V that the mask leaves out become zero: 0 * NaN would not be 0.  A thread per key; both tiles do it, each
+          // before its own P is posted, so that neither's product can be ahead.
           at.next(STAGES);  // K
-          if (t == 0 && (w.x & w.y & w.z & w.w) != 0xffffffffu) {
-            ok = __all_sync(0xffffffffu, bounded_wait(&gb->kv_full[at.stage], at.phase, &gb->abort_flag, status_word, 40));
+          if ((w.x & w.y & w.z & w.w) != 0xffffffffu) {
+            ok = warp_wait(&gb->kv_full[at.stage], at.phase, &gb->abort_flag, status_word, 40);
             if (!ok) break;
             const uint32_t word = (warp & 2) ? ((warp & 1) ? w.w : w.z) : ((warp & 1) ? w.y : w.x);
             if (!((word >> lane) & 1u)) {
@@ -569,8 +538,7 @@ __global__ void __launch_bounds__(XA_THREADS, 1) cross_attention_kernel(const __
         ok = values_done();
         if (!ok) break;
         tcgen05_fence_after();
-        if (pending) ok = write_out();
-        if (!ok) break;
+        if (pending) write_out();
         if (j == 0) {
           m = top;
           l = 0.f;
@@ -590,8 +558,7 @@ __global__ void __launch_bounds__(XA_THREADS, 1) cross_attention_kernel(const __
           }
           tmem_st_wait();
         }
-        // A row of -inf alone has P = 0; one with an infinity becomes NaN whichever way its exponentials are computed.
-        const float mc = m == NEG_INF ? 0.f : m == INFINITY ? NAN : m * p.c;
+        const float mc = m == NEG_INF ? 0.f : m * p.c;  // a row of -inf alone: P = 0
         const uint64_t c2 = xa_pair(p.c, p.c), mc2 = xa_pair(-mc, -mc);
         uint64_t sum2[2] = {0, 0};
 #pragma unroll
@@ -601,13 +568,9 @@ __global__ void __launch_bounds__(XA_THREADS, 1) cross_attention_kernel(const __
           for (int x = 0; x < 16; ++x) {
             uint64_t e = xa_fma2(xa_pair(__uint_as_float(v[q][2 * x]), __uint_as_float(v[q][2 * x + 1])), c2, mc2);
             float lo, hi;
-            if (x % XA_POLY == XA_POLY - 1) {
-              xa_exp2_fma(e, lo, hi);
-            } else {
-              xa_unpair(e, lo, hi);
-              lo = xa_exp2(lo);
-              hi = xa_exp2(hi);
-            }
+            xa_unpair(e, lo, hi);
+            lo = xa_exp2(lo);
+            hi = xa_exp2(hi);
             sum2[x & 1] = xa_add2(sum2[x & 1], xa_pair(lo, hi));
             pk[x] = xa_pack<T>(lo, hi);
           }
@@ -629,14 +592,14 @@ __global__ void __launch_bounds__(XA_THREADS, 1) cross_attention_kernel(const __
       out_row = next_row;
       part_base = next_base;
       out_b = it.b;
-      out_q0 = it.q0 + t * p.q_per_tile;
+      out_q0 = it.q0 + t * p.q_per_tile + (warp & 3) * (p.q_per_tile / 4);
       out_head0 = it.head0;
     }
     if (ok && pending && values_done()) {
       tcgen05_fence_after();
       write_out();
     }
-    if (threadIdx.x % 128 == 0) bulk_wait_group_all();  // the output is written before the CTA retires
+    if (lane == 0) bulk_wait_group_all();  // the output is written before the CTA retires
     __syncwarp();
   }
 
@@ -737,14 +700,14 @@ struct XaPlan {
 };
 static size_t xa_round(size_t n) { return (n + 255) / 256 * 256; }
 
-// Heads of a tile: the largest divisor of the group that fits its 128 rows.  Splits of the key range: items cost their
+// Heads of a tile: the largest power of two up to 32 that divides the group, so that 32 rows, a warp's, are whole
+// queries of all of them.  Splits of the key range: items cost their
 // steps plus about four more for their first loads and their output, a split launch about four for the join; the number
 // of splits is the one whose waves over the SMs cost least.
 static XaPlan xa_plan(int64_t batch, int64_t sq, int64_t skv, int64_t heads, int64_t kv_heads, int64_t d, bool masked, int sms) {
   XaPlan p{};
   const int group = (int)(heads / kv_heads);
-  p.g = group < XA_ROWS ? group : XA_ROWS;
-  while (group % p.g != 0) --p.g;
+  for (p.g = 1; p.g < XA_MAX_GROUP && group % (2 * p.g) == 0;) p.g *= 2;
   p.q_per_tile = XA_ROWS / p.g;
   p.chunks = group / p.g;
   p.q_pairs = (int)((sq + 2 * p.q_per_tile - 1) / (2 * p.q_per_tile));
@@ -856,7 +819,7 @@ extern "C" int cdb_cross_attention(const void* q_v, const void* k_v, const void*
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   XaParams p{};
   if (!xa_map(&p.map_q, bf16, *q, d, heads, sq, batch, plan.g, plan.q_per_tile) ||
-      !xa_map(&p.map_out, bf16, cdb_heads{out, sq * heads * d, heads * d, d}, d, heads, sq, batch, plan.g, plan.q_per_tile) ||
+      !xa_map(&p.map_out, bf16, cdb_heads{out, sq * heads * d, heads * d, d}, d, heads, sq, batch, plan.g, plan.q_per_tile / 4) ||
       !xa_map(&p.map_k, bf16, *k, d, kv_heads, skv, batch, 1, XA_KEYS) || !xa_map(&p.map_v, bf16, *v, d, kv_heads, skv, batch, 1, XA_KEYS)) {
     set_cuda_error(cudaErrorUnknown, "cuTensorMapEncodeTiled");
     return CDB_ERR_CUDA;

@@ -155,21 +155,33 @@ __device__ __forceinline__ void tcgen05_commit_both(uint32_t bar_cta_addr) {
 // Bounded wait for a phase of a barrier: false if the CTA is aborting, or once `limit_ns` passed without it, after
 // which the CTA's abort flag is up and `code` is latched in the caller's status word.
 constexpr uint64_t BARRIER_LIMIT_NS = 2000000000ull;
+__device__ __forceinline__ bool barrier_overdue(uint64_t& t0, volatile int* abort_flag, int32_t* status_word, int code) {
+  if (*abort_flag) return true;
+  const uint64_t now = global_timer_ns();
+  if (t0 == 0) t0 = now;
+  else if (now - t0 > BARRIER_LIMIT_NS) {
+    *abort_flag = 1;
+    if (status_word) atomicCAS(status_word, 0, code);
+    return true;
+  }
+  return false;
+}
 __device__ __forceinline__ bool bounded_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
                                              int32_t* status_word, int code) {
   uint64_t t0 = 0;
   for (uint32_t it = 0;; ++it) {
     if (mbar_try_wait(bar, parity)) return true;
-    if ((it & 255u) == 255u) {
-      if (*abort_flag) return false;
-      const uint64_t now = global_timer_ns();
-      if (t0 == 0) t0 = now;
-      else if (now - t0 > BARRIER_LIMIT_NS) {
-        *abort_flag = 1;
-        if (status_word) atomicCAS(status_word, 0, code);
-        return false;
-      }
-    }
+    if ((it & 255u) == 255u && barrier_overdue(t0, abort_flag, status_word, code)) return false;
+  }
+}
+// The same by a whole, converged warp, with one answer for all lanes.  The vote inside the loop keeps its branch uniform
+// (a satisfied wait takes about 60 clocks; a vote over bounded_wait's results 100).
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int32_t* status_word,
+                                          int code) {
+  uint64_t t0 = 0;
+  for (uint32_t it = 0;; ++it) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    if ((it & 255u) == 255u && __any_sync(0xffffffffu, barrier_overdue(t0, abort_flag, status_word, code))) return false;
   }
 }
 #endif  // __CUDACC__
