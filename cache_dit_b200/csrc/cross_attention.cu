@@ -183,25 +183,6 @@ __device__ __forceinline__ float xa_max3(float a, float b, float c) {  // NaN if
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
-// Two fp32 operations in one instruction.
-__device__ __forceinline__ uint64_t xa_pair(float lo, float hi) {
-  uint64_t d;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
-  return d;
-}
-__device__ __forceinline__ void xa_unpair(uint64_t p, float& lo, float& hi) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(p));
-}
-__device__ __forceinline__ uint64_t xa_fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ uint64_t xa_add2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
 template <typename T>
 __device__ __forceinline__ uint32_t xa_pack(float lo, float hi) {
   if constexpr (__is_same(T, __nv_bfloat16)) {
@@ -559,19 +540,19 @@ __global__ void __launch_bounds__(XA_THREADS, 1) cross_attention_kernel(const __
           tmem_st_wait();
         }
         const float mc = m == NEG_INF ? 0.f : m * p.c;  // a row of -inf alone: P = 0
-        const uint64_t c2 = xa_pair(p.c, p.c), mc2 = xa_pair(-mc, -mc);
+        const uint64_t c2 = f32_pair(p.c, p.c), mc2 = f32_pair(-mc, -mc);
         uint64_t sum2[2] = {0, 0};
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           uint32_t pk[16];
 #pragma unroll
           for (int x = 0; x < 16; ++x) {
-            uint64_t e = xa_fma2(xa_pair(__uint_as_float(v[q][2 * x]), __uint_as_float(v[q][2 * x + 1])), c2, mc2);
+            uint64_t e = f32_fma2(f32_pair(__uint_as_float(v[q][2 * x]), __uint_as_float(v[q][2 * x + 1])), c2, mc2);
             float lo, hi;
-            xa_unpair(e, lo, hi);
+            f32_unpair(e, lo, hi);
             lo = xa_exp2(lo);
             hi = xa_exp2(hi);
-            sum2[x & 1] = xa_add2(sum2[x & 1], xa_pair(lo, hi));
+            sum2[x & 1] = f32_add2(sum2[x & 1], f32_pair(lo, hi));
             pk[x] = xa_pack<T>(lo, hi);
           }
           tmem_st_32x32b_x16(p_addr + q * 16, pk);
@@ -583,7 +564,7 @@ __global__ void __launch_bounds__(XA_THREADS, 1) cross_attention_kernel(const __
           }
         }
         float l0, l1;
-        xa_unpair(xa_add2(sum2[0], sum2[1]), l0, l1);
+        f32_unpair(f32_add2(sum2[0], sum2[1]), l0, l1);
         l += l0 + l1;
         ++posted;
       }

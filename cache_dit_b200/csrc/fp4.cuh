@@ -87,8 +87,9 @@ __device__ __forceinline__ float fp4_row_scale(float top) {
 }
 
 // The scale byte of a block whose largest magnitude is `top`, and how its elements become codes:
-// code = e2m1(q), q = x / step.  nvfp4: q from a reciprocal and one correction (Markstein), which is the correctly
-// rounded quotient; mxfp4: step is a power of two, x * inverse is exact.
+// code = e2m1(q), q = x / step.  nvfp4: q from an approximate reciprocal and one correction, q' = q + (x - q step) inverse:
+// a quotient that is an fp32 number (a rounding boundary is) comes out as that number, any other within a last place,
+// which is all that a decision needs; mxfp4: step is a power of two, x * inverse is exact.
 struct Fp4Step {
   uint32_t byte;
   float step, inverse;
@@ -106,7 +107,8 @@ __device__ __forceinline__ Fp4Step fp4_block_step(float top, float row_scale) {
     s.byte = finite ? float_to_e4m3(t) : 0u;
     const float v = e4m3_to_float(s.byte);
     s.step = v * row_scale;
-    s.inverse = s.byte != 0u ? __frcp_rn(s.step) : 0.f;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s.inverse) : "f"(s.step));
+    if (s.byte == 0u) s.inverse = 0.f;
   } else {
     const uint32_t e = __float_as_uint(top) >> 23;  // top >= 0
     s.byte = e == 255u ? 255u : e > 2u ? e - 2u : 0u;
@@ -115,12 +117,20 @@ __device__ __forceinline__ Fp4Step fp4_block_step(float top, float row_scale) {
   }
   return s;
 }
+// Eight elements of a block -> their codes.
 template <bool NV>
-__device__ __forceinline__ float fp4_quotient(float x, const Fp4Step& s) {
-  const float q = __fmul_rn(x, s.inverse);
-  if constexpr (!NV) return q;
-  // a block of zeros (inverse 0) has step 0: the correction adds x * 0
-  return fmaf(fmaf(-q, s.step, x), s.inverse, q);
+__device__ __forceinline__ uint32_t fp4_codes(const float (&x)[8], const Fp4Step& s) {
+  float q[8];
+  const uint64_t inverse = f32_pair(s.inverse, s.inverse), minus_step = f32_pair(-s.step, -s.step);
+#pragma unroll
+  for (int j = 0; j < 8; j += 2) {
+    const uint64_t v = f32_pair(x[j], x[j + 1]);
+    uint64_t e = f32_mul2(v, inverse);
+    // a block of zeros (inverse 0) has step 0: the correction adds x * 0
+    if constexpr (NV) e = f32_fma2(f32_fma2(e, minus_step, v), inverse, e);
+    f32_unpair(e, q[j], q[j + 1]);
+  }
+  return e2m1x8(q);
 }
 #endif
 

@@ -103,14 +103,27 @@ __global__ void __launch_bounds__(FP4_THREADS)
   const int64_t tiles = fp4_panel_tiles(cols, NV);
   const int64_t all_rows = (rows + 127) & ~(int64_t)127;
   int parity = 0;
-  for (int64_t base = (int64_t)blockIdx.x * ROWS; base < all_rows; base += (int64_t)gridDim.x * ROWS, parity ^= 1) {
-    const int64_t row = base + sub;  // all_rows is a multiple of ROWS
-    Fp4Unit<T> u[UNITS];
+  // 16-bit rows are loaded a row ahead: its loads are in flight while the one before it is reduced and written.
+  constexpr bool AHEAD = sizeof(T) == 2;
+  Fp4Unit<T> ahead[UNITS];
+  auto load = [&](int64_t row, Fp4Unit<T>(&u)[UNITS]) {
 #pragma unroll
     for (int i = 0; i < UNITS; ++i) {
       const int k = t + i * TPR;
       if (row < rows && k < units) u[i].load(x + row * ld_x + (int64_t)k * 16);
       else u[i].zero();
+    }
+  };
+  if (AHEAD) load((int64_t)blockIdx.x * ROWS + sub, ahead);
+  for (int64_t base = (int64_t)blockIdx.x * ROWS; base < all_rows; base += (int64_t)gridDim.x * ROWS, parity ^= 1) {
+    const int64_t row = base + sub;  // all_rows is a multiple of ROWS
+    Fp4Unit<T> u[UNITS];
+    if (AHEAD) {
+#pragma unroll
+      for (int i = 0; i < UNITS; ++i) u[i] = ahead[i];
+      load(row + (int64_t)gridDim.x * ROWS, ahead);
+    } else {
+      load(row, u);
     }
     float top[UNITS];
     float row_top = 0.f;
@@ -142,13 +155,9 @@ __global__ void __launch_bounds__(FP4_THREADS)
       float f[8];
       uint2 c;
       u[i].get(0, f);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = fp4_quotient<NV>(f[j], s);
-      c.x = e2m1x8(f);
+      c.x = fp4_codes<NV>(f, s);
       u[i].get(1, f);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = fp4_quotient<NV>(f[j], s);
-      c.y = e2m1x8(f);
+      c.y = fp4_codes<NV>(f, s);
       const bool live = row < rows && k < units;
       if (live) __stcs(reinterpret_cast<uint2*>(codes + row * (int64_t)(cols >> 1)) + k, c);
       // four scales make one word: four neighbouring lanes (nvfp4), or every other one of eight (mxfp4)
@@ -234,7 +243,7 @@ static int launch_quant(const void* x, int64_t rows, int cols, int64_t ld_x, voi
   return CDB_OK;
 }
 
-// Threads per row: the fewest that hold the row's padded units, four per thread, so that rows of one warp need no
+// Threads per row: the fewest that hold the row's padded units, three to five per thread, so that rows of one warp need no
 // block barrier and a CTA has several rows in flight.  All padded units need a thread: it writes their zero scales.
 template <typename T, bool NV>
 static int dispatch_quant(const void* x, int64_t rows, int cols, int64_t ld_x, void* codes, void* scales,
@@ -245,7 +254,10 @@ static int dispatch_quant(const void* x, int64_t rows, int cols, int64_t ld_x, v
   CDB_Q(32, 1);
   CDB_Q(32, 2);
   CDB_Q(32, 4);
+  CDB_Q(64, 3);
   CDB_Q(64, 4);
+  CDB_Q(64, 5);
+  CDB_Q(128, 3);
   CDB_Q(128, 4);
   CDB_Q(256, 4);
 #undef CDB_Q

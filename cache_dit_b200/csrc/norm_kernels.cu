@@ -34,6 +34,22 @@ __device__ __forceinline__ float to_f(T v) { return (float)v; }
 template <typename T>
 __device__ __forceinline__ T from_f(float v) { return (T)v; }  // round to nearest even
 
+// Eight 16-bit elements of a 16-byte packet.
+template <typename T>
+__device__ __forceinline__ void unpack8(const uint4& v, float (&f)[8]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (__is_same(T, __nv_bfloat16)) {
+      f[2 * i] = __uint_as_float(w[i] << 16);
+      f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    } else {
+      const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      f[2 * i] = t.x;
+      f[2 * i + 1] = t.y;
+    }
+  }
+}
 // Eight consecutive elements; `n` of them exist (the rest read as 0 and are not written).
 template <typename T, bool ALIGNED>
 __device__ __forceinline__ void load8(const T* p, int n, float (&f)[8]) {
@@ -42,19 +58,7 @@ __device__ __forceinline__ void load8(const T* p, int n, float (&f)[8]) {
       const float4 a = *reinterpret_cast<const float4*>(p), b = *(reinterpret_cast<const float4*>(p) + 1);
       f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
     } else {
-      const uint4 v = *reinterpret_cast<const uint4*>(p);
-      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (__is_same(T, __nv_bfloat16)) {
-          f[2 * i] = __uint_as_float(w[i] << 16);
-          f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-        } else {
-          const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-          f[2 * i] = t.x;
-          f[2 * i + 1] = t.y;
-        }
-      }
+      unpack8<T>(*reinterpret_cast<const uint4*>(p), f);
     }
   } else {
 #pragma unroll
@@ -86,6 +90,53 @@ __device__ __forceinline__ void store8(T* p, int n, const float (&f)[8]) {
     for (int i = 0; i < 8; ++i)
       if (i < n) p[i] = from_f<T>(f[i]);
   }
+}
+
+// Rounds eight numbers to T and returns the largest magnitude's bits (as integers: infinity and NaN are above all).
+template <typename T>
+__device__ __forceinline__ uint32_t round8(float (&f)[8]) {
+  if constexpr (sizeof(T) == 4) {
+    uint32_t top = 0u;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(f[j]) & 0x7fffffffu);
+    return top;
+  } else {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (__is_same(T, __nv_bfloat16)) {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&v);
+      } else {
+        const __half2 v = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&v);
+      }
+    }
+    unpack8<T>(make_uint4(w[0], w[1], w[2], w[3]), f);
+    const uint32_t m = __vmaxu2(__vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu), __vmaxu2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
+    const uint32_t top = max(m & 0xffffu, m >> 16);
+    if constexpr (__is_same(T, __nv_bfloat16)) return top << 16;
+    else return __float_as_uint(__half2float(__ushort_as_half((unsigned short)top)));
+  }
+}
+
+// v = a * b + c and friends on eight numbers, two per instruction.
+__device__ __forceinline__ void fma8(float (&v)[8], const float (&a)[8], const float (&b)[8], const float (&c)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; j += 2)
+    f32_unpair(f32_fma2(f32_pair(a[j], a[j + 1]), f32_pair(b[j], b[j + 1]), f32_pair(c[j], c[j + 1])), v[j], v[j + 1]);
+}
+__device__ __forceinline__ void mul8(float (&v)[8], const float (&a)[8], const float (&b)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; j += 2) f32_unpair(f32_mul2(f32_pair(a[j], a[j + 1]), f32_pair(b[j], b[j + 1])), v[j], v[j + 1]);
+}
+__device__ __forceinline__ void add8(float (&v)[8], const float (&a)[8], const float (&b)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; j += 2) f32_unpair(f32_add2(f32_pair(a[j], a[j + 1]), f32_pair(b[j], b[j + 1])), v[j], v[j + 1]);
+}
+__device__ __forceinline__ void fill8(float (&v)[8], float x) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = x;
 }
 
 // Sum (or maximum) over the TPR threads of a row.  `slot` is this reduction's number within the row and the row's
@@ -120,32 +171,54 @@ __device__ __forceinline__ uint32_t row_max(uint32_t v, float* words) {
 }
 
 // The statistics of a row held as v[PACKS][8]: subtracts the mean (LayerNorm) and returns 1 / sqrt(mean square + eps).
-template <int TPR, int PACKS>
+template <int TPR, int PACKS, bool ALIGNED>
 __device__ __forceinline__ float normalise(float (&v)[PACKS][8], int kind, int t, int dim, float eps, float (*words)[NORM_THREADS / 32]) {
   const float inv_dim = 1.0f / (float)dim;
   if (kind == NORM_LAYER) {
-    float s = 0.f;
+    uint64_t s2[2] = {0, 0};
 #pragma unroll
     for (int i = 0; i < PACKS; ++i)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) s += v[i][j];
-    const float mean = row_sum<TPR>(s, words[0]) * inv_dim;
+      for (int j = 0; j < 8; j += 2) s2[(j >> 1) & 1] = f32_add2(s2[(j >> 1) & 1], f32_pair(v[i][j], v[i][j + 1]));
+    float lo, hi;
+    f32_unpair(f32_add2(s2[0], s2[1]), lo, hi);
+    const float mean = row_sum<TPR>(lo + hi, words[0]) * inv_dim;
+    float minus[8];
+    fill8(minus, -mean);
 #pragma unroll
     for (int i = 0; i < PACKS; ++i) {
       const int left = dim - (t + i * TPR) * 8;
+      if constexpr (ALIGNED) {  // a pack is all there or not at all
+        if (left > 0) add8(v[i], v[i], minus);
+      } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] = j < left ? v[i][j] - mean : 0.f;
+        for (int j = 0; j < 8; ++j) v[i][j] = j < left ? v[i][j] - mean : 0.f;
+      }
     }
   }
-  float q = 0.f;
+  uint64_t q2[2] = {0, 0};
 #pragma unroll
   for (int i = 0; i < PACKS; ++i)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) q = fmaf(v[i][j], v[i][j], q);
-  return rsqrtf(fmaf(row_sum<TPR>(q, words[1]), inv_dim, eps));
+    for (int j = 0; j < 8; j += 2) {
+      const uint64_t e = f32_pair(v[i][j], v[i][j + 1]);
+      q2[(j >> 1) & 1] = f32_fma2(e, e, q2[(j >> 1) & 1]);
+    }
+  float lo, hi;
+  f32_unpair(f32_add2(q2[0], q2[1]), lo, hi);
+  return rsqrtf(fmaf(row_sum<TPR>(lo + hi, words[1]), inv_dim, eps));
 }
 
-template <typename T, int TPR, int PACKS, bool ALIGNED>
+// A row's cache lines on their way into L2, one per thread: with a quarter of the warps an SM can hold (a row needs its
+// registers), the loads of the next row would otherwise start only when this one is written.
+template <typename T, int TPR>
+__device__ __forceinline__ void prefetch_row(const T* p, int dim, int t) {
+  for (int c = t * (128 / (int)sizeof(T)); c < dim; c += TPR * (128 / (int)sizeof(T)))
+    asm volatile("prefetch.global.L2 [%0];" ::"l"(p + c));
+}
+
+// POST: the branch is normalised first, so all of it is held at once; without, a pack of it lives only until it is added.
+template <typename T, int TPR, int PACKS, bool ALIGNED, bool POST>
 __global__ void __launch_bounds__(NORM_THREADS) gated_residual_norm_kernel(const __grid_constant__ NormArgs a) {
   pdl_launch_dependents();
   pdl_wait_prior();
@@ -163,6 +236,25 @@ __global__ void __launch_bounds__(NORM_THREADS) gated_residual_norm_kernel(const
   const T* bias = static_cast<const T*>(a.bias);
   const T* post_weight = static_cast<const T*>(a.post_weight);
   const T* post_bias = static_cast<const T*>(a.post_bias);
+  // 16-bit rows without a post norm are loaded a row ahead, into registers: a row's loads are in flight while the one
+  // before it is reduced and written.  Elsewhere the registers are short and the next row only moves into L2.
+  constexpr bool AHEAD = ALIGNED && sizeof(T) == 2 && !POST && PACKS <= 5;
+  uint4 ax[AHEAD ? PACKS : 1], ay[AHEAD ? PACKS : 1];
+  auto load_ahead = [&](int64_t row) {
+    if constexpr (AHEAD) {
+      const int64_t b = row / a.tokens, tok = row - b * a.tokens;
+      const uint4* xr = reinterpret_cast<const uint4*>(static_cast<const T*>(a.x) + b * a.x_batch + tok * a.x_row);
+      const uint4* yr = reinterpret_cast<const uint4*>(static_cast<const T*>(a.y) + b * a.y_batch + tok * a.y_row);
+#pragma unroll
+      for (int i = 0; i < PACKS; ++i) {
+        const int pk = t + i * TPR;
+        const bool in = row < a.rows && pk * 8 < dim;
+        ax[i] = in ? __ldcs(xr + pk) : make_uint4(0, 0, 0, 0);
+        ay[i] = in && a.y != nullptr ? __ldcs(yr + pk) : make_uint4(0, 0, 0, 0);
+      }
+    }
+  };
+  load_ahead((int64_t)blockIdx.x * ROWS + sub);
   int parity = 0;
   for (int64_t row = (int64_t)blockIdx.x * ROWS + sub; row < all_rows; row += (int64_t)gridDim.x * ROWS, parity ^= 1) {
     if (row >= a.rows) {  // padding of the last panel of block scales (the same for all threads of the row)
@@ -171,11 +263,19 @@ __global__ void __launch_bounds__(NORM_THREADS) gated_residual_norm_kernel(const
     }
     const int64_t b = row / a.tokens, tok = row - b * a.tokens;
     const T* xr = static_cast<const T*>(a.x) + b * a.x_batch + tok * a.x_row;
+    const int64_t next = row + (int64_t)gridDim.x * ROWS;
+    if (!AHEAD && next < a.rows) {
+      const int64_t nb = next / a.tokens, nt = next - nb * a.tokens;
+      prefetch_row<T, TPR>(static_cast<const T*>(a.x) + nb * a.x_batch + nt * a.x_row, dim, t);
+      if (a.y != nullptr) prefetch_row<T, TPR>(static_cast<const T*>(a.y) + nb * a.y_batch + nt * a.y_row, dim, t);
+    }
     float v[PACKS][8];
 #pragma unroll
     for (int i = 0; i < PACKS; ++i) {
       const int c = (t + i * TPR) * 8;
-      if (c < dim) {
+      if constexpr (AHEAD) {
+        unpack8<T>(ax[i], v[i]);
+      } else if (c < dim) {
         load8<T, ALIGNED>(xr + c, dim - c, v[i]);
       } else {
 #pragma unroll
@@ -184,89 +284,92 @@ __global__ void __launch_bounds__(NORM_THREADS) gated_residual_norm_kernel(const
     }
     if (a.y != nullptr) {
       const T* yr = static_cast<const T*>(a.y) + b * a.y_batch + tok * a.y_row;
-      float y[PACKS][8];
-#pragma unroll
-      for (int i = 0; i < PACKS; ++i) {
-        const int c = (t + i * TPR) * 8;
-        if (c < dim) {
-          load8<T, ALIGNED>(yr + c, dim - c, y[i]);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) y[i][j] = 0.f;
-        }
-      }
-      float r = 1.f;
-      if (a.post != NORM_NONE) r = normalise<TPR, PACKS>(y, a.post, t, dim, a.post_eps, s_words[parity]);
       T* xo = static_cast<T*>(a.x_out) + row * dim;
+      auto add = [&](int i, int c, const float(&y)[8]) {  // x' of one pack
+        float f[8], alpha[8];
+        fill8(alpha, a.residual_scale);
+        if (gate != nullptr) {
+          load8<T, ALIGNED>(gate + b * a.gate_batch + c, dim - c, f);
+          mul8(f, f, alpha);
+          fma8(v[i], f, y, v[i]);
+        } else {
+          fma8(v[i], alpha, y, v[i]);
+        }
+        store8<T, ALIGNED>(xo + c, dim - c, v[i]);
+      };
+      if constexpr (POST) {
+        float y[PACKS][8];
 #pragma unroll
-      for (int i = 0; i < PACKS; ++i) {
-        const int c = (t + i * TPR) * 8;
-        if (c < dim) {
-          float f[8];
-          if (a.post != NORM_NONE) {
-            if (post_weight != nullptr) {
-              load8<T, ALIGNED>(post_weight + c, dim - c, f);
-#pragma unroll
-              for (int j = 0; j < 8; ++j) y[i][j] *= r * f[j];
-            } else {
-#pragma unroll
-              for (int j = 0; j < 8; ++j) y[i][j] *= r;
-            }
-            if (post_bias != nullptr) {
-              load8<T, ALIGNED>(post_bias + c, dim - c, f);
-#pragma unroll
-              for (int j = 0; j < 8; ++j) y[i][j] += f[j];
-            }
-          }
-          if (gate != nullptr) {
-            load8<T, ALIGNED>(gate + b * a.gate_batch + c, dim - c, f);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[i][j] = fmaf(a.residual_scale * f[j], y[i][j], v[i][j]);
+        for (int i = 0; i < PACKS; ++i) {
+          const int c = (t + i * TPR) * 8;
+          if (c < dim) {
+            load8<T, ALIGNED>(yr + c, dim - c, y[i]);
           } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[i][j] = fmaf(a.residual_scale, y[i][j], v[i][j]);
+            for (int j = 0; j < 8; ++j) y[i][j] = 0.f;
           }
-          store8<T, ALIGNED>(xo + c, dim - c, v[i]);
+        }
+        const float r = normalise<TPR, PACKS, ALIGNED>(y, a.post, t, dim, a.post_eps, s_words[parity]);
+#pragma unroll
+        for (int i = 0; i < PACKS; ++i) {
+          const int c = (t + i * TPR) * 8;
+          if (c < dim) {
+            float f[8];
+            float g[8];
+            fill8(f, r);
+            if (post_weight != nullptr) {
+              load8<T, ALIGNED>(post_weight + c, dim - c, g);
+              mul8(f, f, g);
+            }
+            fill8(g, 0.f);
+            if (post_bias != nullptr) load8<T, ALIGNED>(post_bias + c, dim - c, g);
+            fma8(y[i], y[i], f, g);
+            add(i, c, y[i]);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < PACKS; ++i) {
+          const int c = (t + i * TPR) * 8;
+          if (c < dim) {
+            float y[8];
+            if constexpr (AHEAD) unpack8<T>(ay[i], y);
+            else load8<T, ALIGNED>(yr + c, dim - c, y);
+            add(i, c, y);
+          }
         }
       }
     }
+    load_ahead(next);
     if (a.norm == NORM_NONE) continue;
-    const float r = normalise<TPR, PACKS>(v, a.norm, t, dim, a.eps, s_words[parity] + 2);
+    const float r = normalise<TPR, PACKS, ALIGNED>(v, a.norm, t, dim, a.eps, s_words[parity] + 2);
     uint32_t top[PACKS];
 #pragma unroll
     for (int i = 0; i < PACKS; ++i) {
       const int c = (t + i * TPR) * 8;
       top[i] = 0u;
       if (c < dim) {
-        float f[8];
+        float f[8], g[8];
+        fill8(f, r);
         if (weight != nullptr) {
-          load8<T, ALIGNED>(weight + c, dim - c, f);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) v[i][j] *= r * f[j];
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) v[i][j] *= r;
+          load8<T, ALIGNED>(weight + c, dim - c, g);
+          mul8(f, f, g);
         }
-        if (bias != nullptr) {
-          load8<T, ALIGNED>(bias + c, dim - c, f);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) v[i][j] += f[j];
-        }
+        fill8(g, 0.f);
+        if (bias != nullptr) load8<T, ALIGNED>(bias + c, dim - c, g);
+        fma8(v[i], v[i], f, g);
         if (a.scale != nullptr) {
-          float g[8];
           load8<T, ALIGNED>(static_cast<const T*>(a.scale) + b * a.scale_batch + c, dim - c, f);
           load8<T, ALIGNED>(static_cast<const T*>(a.shift) + b * a.shift_batch + c, dim - c, g);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) v[i][j] = fmaf(v[i][j], 1.f + f[j], g[j]);
+          float one[8];
+          fill8(one, 1.f);
+          add8(f, f, one);
+          fma8(v[i], v[i], f, g);
         }
         if (!quantise) {
           store8<T, ALIGNED>(static_cast<T*>(a.h_out) + row * dim + c, dim - c, v[i]);
         } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            v[i][j] = to_f(from_f<T>(v[i][j]));
-            top[i] = max(top[i], __float_as_uint(v[i][j]) & 0x7fffffffu);
-          }
+          top[i] = round8<T>(v[i]);
         }
       }
     }
@@ -289,10 +392,8 @@ __global__ void __launch_bounds__(NORM_THREADS) gated_residual_norm_kernel(const
       for (int i = 0; i < PACKS; ++i) {
         const int p = t + i * TPR, c = p * 8;
         const Fp4Step s = nv ? fp4_block_step<true>(__uint_as_float(top[i]), row_scale) : fp4_block_step<false>(__uint_as_float(top[i]), 1.f);
-        float f[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = nv ? fp4_quotient<true>(v[i][j], s) : fp4_quotient<false>(v[i][j], s);
-        if (c < dim) __stcs(reinterpret_cast<uint32_t*>(a.codes + row * (int64_t)(dim >> 1)) + p, e2m1x8(f));
+        const uint32_t codes = nv ? fp4_codes<true>(v[i], s) : fp4_codes<false>(v[i], s);
+        if (c < dim) __stcs(reinterpret_cast<uint32_t*>(a.codes + row * (int64_t)(dim >> 1)) + p, codes);
         uint32_t w = c < dim ? s.byte : 0u;
         const int near = nv ? 2 : 4;  // lanes of a block
         w |= __shfl_down_sync(0xffffffffu, w, near) << 8;
@@ -304,17 +405,17 @@ __global__ void __launch_bounds__(NORM_THREADS) gated_residual_norm_kernel(const
   }
 }
 
-template <typename T, int TPR, int PACKS, bool ALIGNED>
+template <typename T, int TPR, int PACKS, bool ALIGNED, bool POST>
 static int launch_norm(const NormArgs& a, cudaStream_t st) {
   static PerDevice resident;
   const int64_t per_sm = resident.get([]() -> int64_t {
     int n = 0;
-    cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, gated_residual_norm_kernel<T, TPR, PACKS, ALIGNED>, NORM_THREADS, 0);
+    cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, gated_residual_norm_kernel<T, TPR, PACKS, ALIGNED, POST>, NORM_THREADS, 0);
     return n > 0 ? n : 1;
   });
   const int64_t rows = a.format >= 0 ? (a.rows + 127) / 128 * 128 : a.rows;
   const int64_t want = (rows + NORM_THREADS / TPR - 1) / (NORM_THREADS / TPR), cap = per_sm * sm_count();
-  CDB_CUDA_CHECK(launch_pdl(gated_residual_norm_kernel<T, TPR, PACKS, ALIGNED>, dim3((unsigned)(want < cap ? want : cap)),
+  CDB_CUDA_CHECK(launch_pdl(gated_residual_norm_kernel<T, TPR, PACKS, ALIGNED, POST>, dim3((unsigned)(want < cap ? want : cap)),
                             dim3(NORM_THREADS), 0, st, a));
   return CDB_OK;
 }
@@ -325,7 +426,7 @@ static int dispatch_norm(const NormArgs& a, bool aligned, cudaStream_t st) {
   // with 4-bit output the padded block scales need a thread each
   const int packs = a.format >= 0 ? (a.dim + FP4_STEP_COLS - 1) / FP4_STEP_COLS * (FP4_STEP_COLS / 8) : (a.dim + 7) / 8;
 #define CDB_N(TPR, PACKS, ALIGNED) \
-  if (packs <= TPR * PACKS) return launch_norm<T, TPR, PACKS, ALIGNED>(a, st)
+  if (packs <= TPR * PACKS) return a.post != NORM_NONE ? launch_norm<T, TPR, PACKS, ALIGNED, true>(a, st) : launch_norm<T, TPR, PACKS, ALIGNED, false>(a, st)
   if (aligned) {
     CDB_N(32, 1, true);
     CDB_N(32, 2, true);
