@@ -21,7 +21,7 @@ from .caching import (BasicCacheConfig, BlockAdapter, BlockGraphRunner, disable_
                       load_options, load_parallelism_config, load_quantize_config, refresh_context, steps_mask,
                       supported_pipelines)
 from .distributed import ParallelismBackend, ParallelismConfig, enable_parallelism
-from .quantization import (Float4Rows, Float8RowwiseLinear, QuantizeBackend, QuantizeConfig, float4_dequantize_rows,
+from .quantization import (Float4Linear, Float4Rows, Float8RowwiseLinear, QuantizeBackend, QuantizeConfig, float4_dequantize_rows,
                            float4_linear, float4_quantize_rows, float4_scaled_mm, quantize)
 from .summary import CacheStats, strify, summary
 from . import synthetic  # registers the block adapters of the DiT stand-ins

@@ -187,7 +187,7 @@ __global__ void __launch_bounds__(FP4_THREADS)
   const int64_t total = rows * units;
   const int64_t stride = (int64_t)gridDim.x * FP4_THREADS;
   for (int64_t i = (int64_t)blockIdx.x * FP4_THREADS + threadIdx.x; i < total; i += stride) {
-    const int64_t row = i / units;
+    const int64_t row = total <= UINT32_MAX ? (int64_t)((uint32_t)i / (uint32_t)units) : i / units;
     const int k = (int)(i - row * units);
     const uint2 c = __ldcs(reinterpret_cast<const uint2*>(codes) + i);
     const int b = NV ? k : k >> 1;

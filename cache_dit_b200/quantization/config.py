@@ -1,8 +1,9 @@
 """Quantization config with the reference's field names
 (src/cache_dit/quantization/config.py:329-705).
 
-Only the path this package accelerates is implemented: `quant_type="float8_per_row"` (dynamic
-per-token e4m3 activations x per-output-row e4m3 weights).  Unlike the reference, constructing the
+Implemented: `quant_type="float8_per_row"` (dynamic per-token e4m3 activations x per-output-row e4m3 weights) and the two
+4-bit microscaled types "nvfp4_per_row" (the reference's "nvfp4" with a second-level scale per row instead of per
+tensor) and "mxfp4" (cache_dit_b200/quantization/float4.py).  Unlike the reference, constructing the
 config does not require torchao: the kernels are this package's own.
 """
 from __future__ import annotations
@@ -11,7 +12,7 @@ import dataclasses
 from enum import Enum
 from typing import Any, Callable, Dict, List, Optional, Union
 
-SUPPORTED_QUANT_TYPES = ("float8_per_row", )
+SUPPORTED_QUANT_TYPES = ("float8_per_row", "nvfp4_per_row", "mxfp4")
 KNOWN_QUANT_TYPES = ("float8_per_tensor", "float8_per_row", "float8_per_block", "float8_weight_only", "nvfp4",
                      "nvfp4_weight_only", "int8_per_tensor", "int8_per_row", "int8_weight_only",
                      "int4_weight_only")

@@ -215,3 +215,49 @@ def float4_linear(x: torch.Tensor, w: Float4Rows, bias: Optional[torch.Tensor] =
     x2, ld = _as_matrix(x, rows, cols)
     _native.fp4_linear(x2, ld, _aligned(w)._triple(), bias, out, rows, cols, w.format, gelu)
   return out
+
+
+class Float4Linear(torch.nn.Module):
+  """y = float4_linear(x, W): an nn.Linear replacement with 4-bit activations and weights, bfloat16 in and out.  The weight
+  is quantised once; codes and scales are buffers, so they move and save with the module."""
+
+  def __init__(self, weight: Float4Rows, bias: Optional[torch.Tensor]):
+    super().__init__()
+    self.out_features, self.in_features = weight.shape
+    self.format = weight.format
+    self.register_buffer("weight_codes", weight.codes)                # [N, K / 2] uint8
+    self.register_buffer("weight_block_scales", weight.block_scales)  # tiled, uint8
+    self.register_buffer("weight_row_scale", weight.row_scale)        # [N] float32, None for mxfp4
+    self.register_buffer("bias", bias)                                # [N] bfloat16 or None
+
+  @classmethod
+  def from_linear(cls, linear: torch.nn.Linear, format: str = "nvfp4") -> "Float4Linear":
+    w = linear.weight.detach()
+    if not w.is_cuda:
+      raise RuntimeError("4-bit quantization runs on the GPU: move the module to CUDA first")
+    if not cls.supports(linear):
+      raise RuntimeError("a 4-bit linear needs bfloat16 weights with in_features % 32 == 0, at most "
+                         f"{_native.FP4_MAX_COLS}, and out_features % 8 == 0, got {w.dtype} {tuple(w.shape)}")
+    bias = None if linear.bias is None else linear.bias.detach().to(torch.bfloat16).contiguous()
+    return cls(float4_quantize_rows(w, format), bias)
+
+  @staticmethod
+  def supports(linear: torch.nn.Linear) -> bool:
+    n, k = linear.weight.shape
+    return linear.weight.dtype == torch.bfloat16 and k % 32 == 0 and 0 < k <= _native.FP4_MAX_COLS and n % 8 == 0 and n > 0
+
+  @property
+  def weight_rows(self) -> Float4Rows:
+    return Float4Rows(self.weight_codes, self.weight_block_scales, self.weight_row_scale, self.format, self.in_features)
+
+  def forward_quantized(self, a: Float4Rows, gelu: bool = False) -> torch.Tensor:
+    """Product for activations that a producer already wrote in 4 bits.  `gelu`: the tanh-GELU of the output."""
+    return float4_scaled_mm(a, self.weight_rows, self.bias, torch.bfloat16, gelu)
+
+  def forward(self, x: torch.Tensor, gelu: bool = False) -> torch.Tensor:
+    if x.dtype != torch.bfloat16:
+      x = x.to(torch.bfloat16)
+    return float4_linear(x, self.weight_rows, self.bias, gelu)
+
+  def extra_repr(self) -> str:
+    return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}, 4-bit={self.format}"

@@ -1,4 +1,4 @@
-"""`quantize(module, QuantizeConfig)`: swap eligible nn.Linear layers for FP8 row-wise linears.
+"""`quantize(module, QuantizeConfig)`: swap eligible nn.Linear layers for FP8 row-wise or 4-bit linears.
 
 Layer selection follows the reference's filter (src/cache_dit/quantization/torchao/quantize_ao.py:74-163,
 666-775): inside the repeated transformer block classes only (regional quantization), names not
@@ -12,14 +12,26 @@ from typing import List
 import torch
 
 from .config import QuantizeConfig
+from .float4 import QUANT_TYPES as FLOAT4_TYPES, Float4Linear
 from .linear import Float8RowwiseLinear
 
 logger = logging.getLogger("cache_dit_b200")
 
 
+def _linear_kind(cfg: QuantizeConfig):
+  return Float4Linear if cfg.quant_type in FLOAT4_TYPES else Float8RowwiseLinear
+
+
+def _convert(m: torch.nn.Linear, cfg: QuantizeConfig) -> torch.nn.Module:
+  if cfg.quant_type in FLOAT4_TYPES:
+    return Float4Linear.from_linear(m, FLOAT4_TYPES[cfg.quant_type])
+  return Float8RowwiseLinear.from_linear(m)
+
+
 def _eligible(name: str, m: torch.nn.Module, cfg: QuantizeConfig, skipped: List[str]) -> bool:
   if not isinstance(m, torch.nn.Linear) or isinstance(m, Float8RowwiseLinear):
     return False
+  kind = _linear_kind(cfg)
   if cfg.filter_fn is not None:
     return bool(cfg.filter_fn(m, name))
   for pattern in (cfg.exclude_layers or []):
@@ -29,7 +41,7 @@ def _eligible(name: str, m: torch.nn.Module, cfg: QuantizeConfig, skipped: List[
   if m.weight.dtype != torch.bfloat16:
     skipped.append(f"skip: {name} -> pattern<dtype({m.weight.dtype})!=bfloat16>")
     return False
-  if not Float8RowwiseLinear.supports(m):
+  if not kind.supports(m):
     skipped.append(f"skip: {name} -> pattern<shape{tuple(m.weight.shape)}>")
     return False
   return True
@@ -40,7 +52,7 @@ def _swap_linears(root: torch.nn.Module, prefix: str, cfg: QuantizeConfig, skipp
   for child_name, child in list(root.named_children()):
     full = f"{prefix}.{child_name}" if prefix else child_name
     if _eligible(full, child, cfg, skipped):
-      setattr(root, child_name, Float8RowwiseLinear.from_linear(child))
+      setattr(root, child_name, _convert(child, cfg))
       count += 1
     else:
       count += _swap_linears(child, full, cfg, skipped)

@@ -17,12 +17,26 @@ import torch.nn.functional as F
 from torch import nn
 
 from .. import _native
+from ..block_ops import cross_attention, gated_residual_norm
+from ..quantization.float4 import Float4Linear
 from ..quantization.linear import (Float8RowwiseLinear, _members_share_storage, fused_group, grouped_forward_quantized,
                                    quantize_rows_fused, quantize_rows_fused_pair)
 
 
 def _all_fp8(linears: Sequence[nn.Module]) -> bool:
   return all(isinstance(l, Float8RowwiseLinear) for l in linears)
+
+
+def _float4_format(linears: Sequence[nn.Module]) -> Optional[str]:
+  """The 4-bit format that all of these linears share, or None."""
+  if linears and all(isinstance(l, Float4Linear) for l in linears) and len({l.format for l in linears}) == 1:
+    return linears[0].format
+  return None
+
+
+def _float4_outputs(h, linears: Sequence[nn.Module], gelu_last: bool) -> List[torch.Tensor]:
+  """[lin(h) for lin in linears] of 4-bit rows, the last with its tanh-GELU if wanted."""
+  return [l.forward_quantized(h, gelu_last and l is linears[-1]) for l in linears]
 
 
 def gelu_in_product() -> bool:
@@ -42,11 +56,54 @@ def norm_modulate_linears(x: torch.Tensor, shift: torch.Tensor, scale: torch.Ten
     if len(linears) > 1:  # one GEMM over the concatenated output rows
       return list(fused_group(linears).forward_quantized(a_q, a_scale, lead, gelu_last))
     return [linears[0].forward_quantized(a_q, a_scale, lead, gelu_last)]
+  fmt = _float4_format(linears)
+  if fmt is not None and x.is_cuda and not torch.is_grad_enabled():
+    _, h = gated_residual_norm(x, norm="layer", scale=scale, shift=shift, eps=eps, quantize=fmt)
+    return _float4_outputs(h, linears, gelu_last)
   y = F.layer_norm(x, (x.shape[-1], ), eps=eps) * (1 + scale[:, None]) + shift[:, None]
   outs = [l(y) for l in linears]
   if gelu_last:
     outs[-1] = F.gelu(outs[-1], approximate="tanh")
   return outs
+
+
+def gated_add_norm_modulate_linears(x: torch.Tensor, gate: Optional[torch.Tensor], y: torch.Tensor, shift: torch.Tensor,
+                                    scale: torch.Tensor, linears: Sequence[nn.Module], eps: float = 1e-6,
+                                    gelu_last: bool = False):
+  """(x', [lin(LayerNorm(x') * (1 + scale) + shift) for lin in linears]) with x' = x + gate[:, None] * y (gate None: x + y).
+  With 4-bit linears one kernel adds, normalises and writes the linears' 4-bit input."""
+  fmt = _float4_format(linears)
+  if fmt is not None and x.is_cuda and not torch.is_grad_enabled():
+    x, h = gated_residual_norm(x, y, gate, norm="layer", scale=scale, shift=shift, eps=eps, quantize=fmt)
+    return x, _float4_outputs(h, linears, gelu_last)
+  x = x + y if gate is None else gated_add(x, gate, y)
+  return x, norm_modulate_linears(x, shift, scale, linears, eps, gelu_last)
+
+
+def gated_add_layer_norm_linear(x: torch.Tensor, gate: torch.Tensor, y: torch.Tensor, norm: nn.LayerNorm, linear: nn.Module):
+  """(x', linear(norm(x'))) with x' = x + gate[:, None] * y; one kernel for all but the product with a 4-bit linear."""
+  fmt = _float4_format((linear, ))
+  if fmt is not None and x.is_cuda and not torch.is_grad_enabled():
+    x, h = gated_residual_norm(x, y, gate, norm="layer", weight=norm.weight, bias=norm.bias, eps=norm.eps, quantize=fmt)
+    return x, linear.forward_quantized(h)
+  x = gated_add(x, gate, y)
+  return x, linear(norm(x))
+
+
+def encoder_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, key_mask: Optional[torch.Tensor] = None) -> torch.Tensor:
+  """Attention of q [B, S, H, D] to an encoder's k, v [B, T, H, D]; key_mask bool [B, T] names the tokens of each prompt
+  (a batch of prompts padded to one length).  Masked prompts go through this package's kernel on the GPU; without a mask
+  the library's attention runs, as it does for self-attention."""
+  if key_mask is None:
+    return F.scaled_dot_product_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2)).transpose(1, 2)
+  if q.is_cuda and q.dtype in (torch.bfloat16, torch.float16) and not torch.is_grad_enabled():
+    return cross_attention(q, k, v, key_mask)
+  keep = key_mask[:, None, None, :]
+  v = torch.where(key_mask[:, :, None, None], v, torch.zeros_like(v))
+  scores = (q.transpose(1, 2).float() @ k.permute(0, 2, 3, 1).float()) * q.shape[-1]**-0.5
+  p = torch.softmax(scores.masked_fill(~keep, float("-inf")), dim=-1)
+  p = torch.where(keep.any(dim=-1, keepdim=True), p, torch.zeros_like(p)).to(v.dtype)  # a prompt without tokens: zeros
+  return (p @ v.transpose(1, 2)).transpose(1, 2)
 
 
 # ---- two streams at once -----------------------------------------------------------------------------

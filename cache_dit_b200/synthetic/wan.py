@@ -23,7 +23,8 @@ from torch import nn
 from ..caching.block_adapters import BlockAdapter, BlockAdapterRegister
 from ..caching.forward_pattern import ForwardPattern
 from .context_parallel import ContextParallelMixin
-from .layers import (RMSNorm, TimestepMLP, UlyssesGroup, gated_add, gelu_in_product, gelu_linear, joint_attention, norm_modulate,
+from .layers import (RMSNorm, TimestepMLP, UlyssesGroup, encoder_attention, gated_add, gated_add_layer_norm_linear,
+                     gated_add_norm_modulate_linears, gelu_in_product, gelu_linear, joint_attention, norm_modulate,
                      norm_modulate_linears, RopeCache, timestep_embedding)
 from .qwen_image import QwenFeedForward
 
@@ -50,24 +51,24 @@ class WanTransformerBlock(nn.Module):
     self.ffn = QwenFeedForward(dim, ffn_dim)
     self.cp: Optional[UlyssesGroup] = None
 
-  def forward(self, hidden_states, encoder_hidden_states, temb, rotary_emb):
+  def forward(self, hidden_states, encoder_hidden_states, temb, rotary_emb, encoder_attention_mask=None):
     mod = (self.scale_shift_table.to(temb.dtype) + temb)  # [B, 6, C]
     shift_msa, scale_msa, gate_msa, c_shift, c_scale, c_gate = mod.unbind(dim=1)
     # 1. self-attention over the video tokens
     a = self.attn1
     q, k, v = norm_modulate_linears(hidden_states, shift_msa, scale_msa, (a.to_q, a.to_k, a.to_v))
     o = joint_attention(((q, a.norm_q), ), ((k, a.norm_k), ), (v, ), rotary_emb, a.heads, self.cp, across_heads=True)
-    hidden_states = gated_add(hidden_states, gate_msa, a.to_out[0](o))
     # 2. cross-attention to the text (local under context parallelism)
-    a = self.attn2
-    q = a.norm_q(a.to_q(self.norm2(hidden_states))).unflatten(-1, (a.heads, a.head_dim))
+    o, a = a.to_out[0](o), self.attn2
+    hidden_states, q = gated_add_layer_norm_linear(hidden_states, gate_msa, o, self.norm2, a.to_q)
+    q = a.norm_q(q).unflatten(-1, (a.heads, a.head_dim))
     k = a.norm_k(a.to_k(encoder_hidden_states)).unflatten(-1, (a.heads, a.head_dim))
     v = a.to_v(encoder_hidden_states).unflatten(-1, (a.heads, a.head_dim))
-    o = F.scaled_dot_product_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2)).transpose(1, 2)
-    hidden_states = hidden_states + a.to_out[0](o.flatten(2))
+    o = encoder_attention(q, k, v, encoder_attention_mask)
     # 3. feed-forward
     act = gelu_in_product()
-    (h, ) = norm_modulate_linears(hidden_states, c_shift, c_scale, (self.ffn.net[0].proj, ), gelu_last=act)
+    hidden_states, (h, ) = gated_add_norm_modulate_linears(hidden_states, None, a.to_out[0](o.flatten(2)), c_shift, c_scale,
+                                                           (self.ffn.net[0].proj, ), gelu_last=act)
     return gated_add(hidden_states, c_gate, gelu_linear(h, self.ffn.net[2], activated=act))
 
 
@@ -96,7 +97,7 @@ class WanTransformer3DModel(ContextParallelMixin, nn.Module):
   def _cp_blocks(self):
     return list(self.blocks)
 
-  def forward(self, hidden_states, encoder_hidden_states, timestep, video_ids):
+  def forward(self, hidden_states, encoder_hidden_states, timestep, video_ids, encoder_attention_mask=None):
     n_tokens = hidden_states.shape[1]
     hidden_states, video_ids = self.cp_shard(hidden_states, 1), self.cp_shard(video_ids, 0)
     dt = hidden_states.dtype
@@ -105,8 +106,9 @@ class WanTransformer3DModel(ContextParallelMixin, nn.Module):
     temb6 = self.time_proj(F.silu(temb)).unflatten(1, (6, -1))
     encoder_hidden_states = self.text_embedder(encoder_hidden_states)
     rope = self._rope_cache.get((video_ids, ), self.axes_dims_rope, dt)
+    mask = () if encoder_attention_mask is None else (encoder_attention_mask, )  # which text tokens each prompt has
     for block in self.blocks:
-      hidden_states = block(hidden_states, encoder_hidden_states, temb6, rope)
+      hidden_states = block(hidden_states, encoder_hidden_states, temb6, rope, *mask)
     shift, scale = (self.scale_shift_table.to(dt) + temb[:, None]).unbind(dim=1)
     out = self.proj_out(norm_modulate(hidden_states, shift, scale))
     return self.cp_gather(out, 1, n_tokens)
