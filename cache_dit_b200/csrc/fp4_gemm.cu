@@ -12,7 +12,7 @@
 //     columns leave no room for the scales (512 columns in all): at bn = 256 the second starts at column 160 and the
 //     two share 96 columns.  The epilogue reads those 96 columns into registers first and hands them over; all that
 //     the next tile's MMAs wait for is that read.
-//   * M <= 4 rows: no tile; the weights are streamed once by the CUDA cores (fp4_gemv_kernel).
+//   * one row: no tile; the weights are streamed once by the CUDA cores (fp4_gemv_kernel).
 //
 // Warp roles (224 threads): warp 0 = TMA producer, warp 1 = tensor memory owner and MMA issuer, warps 2..5 = epilogue,
 // warp 6 = block scales to tensor memory.
@@ -482,59 +482,52 @@ __global__ void __launch_bounds__(F4_THREADS, 1) fp4_gemm_kernel(const __grid_co
   }
 }
 
-// ---- few rows -----------------------------------------------------------------------------------------------
-// M <= 4: a 128-row tile would be padding, and the weights (N * K * 9/16 bytes) are all there is to read.  A warp owns
-// the four columns n, n + 32, n + 64, n + 96 whose block scales share 16 bytes; a lane takes 64 columns of K at a time:
-// 32 bytes of codes of each, one 16-byte load of scales, and the activations, from shared memory, once for all four.
-// The sixteen products of a block are multiples of 0.25 and at most 36: eight of them sum exactly in f16 (at most 288),
-// so the two halves of a packed f16 accumulator hold a block's sum exactly; blocks are summed in fp32.
+// ---- one row ------------------------------------------------------------------------------------------------
+// M = 1: a 128-row tile would be padding, and the weights (N * K * 9/16 bytes) are all there is to read.  A warp owns the
+// four columns n, n + 32, n + 64, n + 96 whose block scales share 16 bytes; a lane takes 32 columns of K at a time: 16
+// bytes of codes of each, one 16-byte load of scales, and the activations, from shared memory, once for all four.  The
+// products of a block of 16 are multiples of 0.25 and at most 36: eight of them sum exactly in f16 (at most 288), so the two
+// halves of a packed f16 accumulator hold the sum exactly; blocks are summed in fp32.
+// From two rows on the tile kernels are faster (4 x 30720 x 5120: 29 us against 50 us of this kernel with four rows).
 constexpr int F4V_THREADS = 256;
-constexpr int F4V_MAX_M = 4;
-constexpr int F4V_SMEM_LIMIT = 96 * 1024;
-__host__ __device__ constexpr int f4v_row_bytes(int pieces) { return pieces * (128 + 16); }  // f16 codes and 4 fp32 scales
+__host__ __device__ constexpr size_t f4v_smem(int chunks) { return (size_t)chunks * (64 + 8); }  // f16 codes, two fp32 scales
 
+// Scales of the two blocks of 16 of a chunk of 32 columns, from the word that holds its four (nvfp4: of 64 columns, mxfp4:
+// of 128).
 template <bool NV>
-__device__ __forceinline__ void piece_scales(uint32_t word, int c, float (&s)[4]) {  // of the blocks of 16 of a piece
+__device__ __forceinline__ float2 chunk_scales(uint32_t word, int c) {
   if constexpr (NV) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) s[i] = e4m3_to_float((word >> (8 * i)) & 0xffu);
+    const uint32_t two = (c & 1) ? word >> 16 : word;
+    return make_float2(e4m3_to_float(two & 0xffu), e4m3_to_float((two >> 8) & 0xffu));
   } else {
-    word >>= (c & 1) * 16;
-    s[0] = s[1] = e8m0_to_float(word & 0xffu);
-    s[2] = s[3] = e8m0_to_float((word >> 8) & 0xffu);
+    const float s = e8m0_to_float((word >> ((c & 3) * 8)) & 0xffu);
+    return make_float2(s, s);
   }
 }
 
-template <int TM, bool NV, typename T>
+template <bool NV, typename T>
 __global__ void __launch_bounds__(F4V_THREADS)
     fp4_gemv_kernel(const uint8_t* __restrict__ a_codes, const uint8_t* __restrict__ a_scales, const float* __restrict__ ra,
                     const uint8_t* __restrict__ w_codes, const uint8_t* __restrict__ w_scales, const float* __restrict__ rw,
-                    const T* __restrict__ bias, T* __restrict__ out, int64_t ld_out, int N, int K, int gelu) {
+                    const T* __restrict__ bias, T* __restrict__ out, int N, int K, int gelu) {
   pdl_launch_dependents();
   pdl_wait_prior();
   extern __shared__ __align__(16) uint8_t smem_raw[];
-  const int pieces = (K + 63) >> 6;  // of 64 columns; the last may be half
-  const int chunks = K >> 5;         // of 32 columns = 16 bytes of codes
+  constexpr int PER_WORD = NV ? 1 : 2;  // log2 of the chunks whose scales share a word
+  const int chunks = K >> 5;            // of 32 columns = 16 bytes of codes
   const int64_t tiles = fp4_panel_tiles(K, NV);
-  uint4* s_a = reinterpret_cast<uint4*>(smem_raw);                         // [TM][8][pieces]: 8 f16 codes each
-  float4* s_s = reinterpret_cast<float4*>(s_a + (size_t)TM * 8 * pieces);  // [TM][pieces]: scales of its 4 blocks of 16
-  for (int i = threadIdx.x; i < TM * pieces * 2; i += F4V_THREADS) {  // i = (m, piece, half)
-    const int m = i / (2 * pieces), h = i - m * 2 * pieces, c = h >> 1, half = h & 1;
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (h < chunks) v = *(reinterpret_cast<const uint4*>(a_codes + (int64_t)m * (K >> 1)) + h);
+  uint4* s_a = reinterpret_cast<uint4*>(smem_raw);             // [4][chunks]: 8 f16 codes each
+  float2* s_s = reinterpret_cast<float2*>(s_a + 4 * chunks);   // [chunks]
+  for (int c = threadIdx.x; c < chunks; c += F4V_THREADS) {
+    const uint4 v = *(reinterpret_cast<const uint4*>(a_codes) + c);
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       uint32_t f[4];
       e2m1x8_to_half2(w[j], f);
-      s_a[(m * 8 + half * 4 + j) * pieces + c] = make_uint4(f[0], f[1], f[2], f[3]);
+      s_a[j * chunks + c] = make_uint4(f[0], f[1], f[2], f[3]);
     }
-    if (half == 0) {
-      const uint32_t word = *reinterpret_cast<const uint32_t*>(a_scales + fp4_scale_word(m, NV ? c : c >> 1, tiles));
-      float s[4];
-      piece_scales<NV>(word, c, s);
-      s_s[m * pieces + c] = make_float4(s[0], s[1], s[2], s[3]);
-    }
+    s_s[c] = chunk_scales<NV>(*reinterpret_cast<const uint32_t*>(a_scales + fp4_scale_word(0, c >> PER_WORD, tiles)), c);
   }
   __syncthreads();
   const int lane = threadIdx.x & 31;
@@ -543,78 +536,55 @@ __global__ void __launch_bounds__(F4V_THREADS)
   const int groups = ((N + 127) >> 7) * 32;
   for (int g = warp; g < groups; g += nwarps) {
     const int n0 = (g >> 5) * 128 + (g & 31);
-    float acc[4][TM];
+    const uint4* wrow[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < 4; ++j) wrow[j] = reinterpret_cast<const uint4*>(w_codes + (int64_t)min(n0 + 32 * j, N - 1) * (K >> 1));
+    const uint8_t* srow = w_scales + fp4_scale_word(n0, 0, tiles);
+    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 2
+    for (int c = lane; c < chunks; c += 32) {
+      const uint4 sw = __ldg(reinterpret_cast<const uint4*>(srow + (c >> PER_WORD) * 512));
+      uint4 wv[4];
 #pragma unroll
-      for (int m = 0; m < TM; ++m) acc[j][m] = 0.f;
-    for (int c = lane; c < pieces; c += 32) {
-      const uint4 sw = __ldg(reinterpret_cast<const uint4*>(w_scales + fp4_scale_word(n0, NV ? c : c >> 1, tiles)));
+      for (int j = 0; j < 4; ++j) wv[j] = __ldcs(wrow[j] + c);
+      const float2 as = s_s[c];
+      uint4 av[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) av[j] = s_a[j * chunks + c];
       const uint32_t sword[4] = {sw.x, sw.y, sw.z, sw.w};
-      uint4 wv[4][2];
+      auto h2 = [](const uint32_t& u) { return *reinterpret_cast<const __half2*>(&u); };
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int n = n0 + 32 * j;
-        const uint4* wrow = reinterpret_cast<const uint4*>(w_codes + (int64_t)n * (K >> 1));
-        wv[j][0] = n < N ? __ldcs(wrow + 2 * c) : make_uint4(0, 0, 0, 0);
-        wv[j][1] = n < N && 2 * c + 1 < chunks ? __ldcs(wrow + 2 * c + 1) : make_uint4(0, 0, 0, 0);
-      }
-      float as[TM][4];
+        const float2 ws = chunk_scales<NV>(sword[j], c);
+        const uint32_t word[4] = {wv[j].x, wv[j].y, wv[j].z, wv[j].w};
 #pragma unroll
-      for (int m = 0; m < TM; ++m) {
-        const float4 t = s_s[m * pieces + c];
-        as[m][0] = t.x; as[m][1] = t.y; as[m][2] = t.z; as[m][3] = t.w;
-      }
-      float ws[4][4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) piece_scales<NV>(sword[j], c, ws[j]);
-#pragma unroll
-      for (int b = 0; b < 4; ++b) {  // blocks of 16: two 16-byte reads of activations, 8 bytes of each column's codes
-        uint4 av[TM][2];
-#pragma unroll
-        for (int m = 0; m < TM; ++m) {
-          av[m][0] = s_a[(m * 8 + 2 * b) * pieces + c];
-          av[m][1] = s_a[(m * 8 + 2 * b + 1) * pieces + c];
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint4 q = wv[j][b >> 1];
+        for (int b = 0; b < 2; ++b) {
           uint32_t f0[4], f1[4];
-          e2m1x8_to_half2((b & 1) ? q.z : q.x, f0);
-          e2m1x8_to_half2((b & 1) ? q.w : q.y, f1);
-          auto h2 = [](const uint32_t& u) { return *reinterpret_cast<const __half2*>(&u); };
-#pragma unroll
-          for (int m = 0; m < TM; ++m) {
-            __half2 t = __hmul2(h2(f0[0]), h2(av[m][0].x));
-            t = __hfma2(h2(f0[1]), h2(av[m][0].y), t);
-            t = __hfma2(h2(f0[2]), h2(av[m][0].z), t);
-            t = __hfma2(h2(f0[3]), h2(av[m][0].w), t);
-            t = __hfma2(h2(f1[0]), h2(av[m][1].x), t);
-            t = __hfma2(h2(f1[1]), h2(av[m][1].y), t);
-            t = __hfma2(h2(f1[2]), h2(av[m][1].z), t);
-            t = __hfma2(h2(f1[3]), h2(av[m][1].w), t);
-            const float2 d = __half22float2(t);
-            acc[j][m] = fmaf(d.x + d.y, ws[j][b] * as[m][b], acc[j][m]);
-          }
+          e2m1x8_to_half2(word[2 * b], f0);
+          e2m1x8_to_half2(word[2 * b + 1], f1);
+          __half2 t = __hmul2(h2(f0[0]), h2(av[2 * b].x));
+          t = __hfma2(h2(f0[1]), h2(av[2 * b].y), t);
+          t = __hfma2(h2(f0[2]), h2(av[2 * b].z), t);
+          t = __hfma2(h2(f0[3]), h2(av[2 * b].w), t);
+          t = __hfma2(h2(f1[0]), h2(av[2 * b + 1].x), t);
+          t = __hfma2(h2(f1[1]), h2(av[2 * b + 1].y), t);
+          t = __hfma2(h2(f1[2]), h2(av[2 * b + 1].z), t);
+          t = __hfma2(h2(f1[3]), h2(av[2 * b + 1].w), t);
+          const float2 d = __half22float2(t);
+          acc[j] = fmaf(d.x + d.y, b ? ws.y * as.y : ws.x * as.x, acc[j]);
         }
       }
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int m = 0; m < TM; ++m) acc[j][m] = warp_sum(acc[j][m]);
+    for (int j = 0; j < 4; ++j) acc[j] = warp_sum(acc[j]);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {  // lane j writes column j
       const int n = n0 + 32 * j;
       if (lane == j && n < N) {
         const float cs = rw != nullptr ? __ldg(rw + n) : 1.f;
-        const float b = bias != nullptr ? (float)bias[n] : 0.f;
-#pragma unroll
-        for (int m = 0; m < TM; ++m) {
-          float v = fmaf(acc[j][m] * (ra != nullptr ? __ldg(ra + m) : 1.f), cs, b);
-          if (gelu) v = gelu_tanh(v);
-          out[(int64_t)m * ld_out + n] = (T)v;
-        }
+        float v = fmaf(acc[j] * (ra != nullptr ? __ldg(ra) : 1.f), cs, bias != nullptr ? (float)bias[n] : 0.f);
+        if (gelu) v = gelu_tanh(v);
+        out[n] = (T)v;
       }
     }
   }
@@ -697,38 +667,21 @@ struct F4Matrix {  // mirrors `cdb_fp4_matrix` of the public header
 };
 
 template <bool NV, typename T>
-static int f4_gemv(const F4Matrix& a, const F4Matrix& w, const void* bias, void* out, int64_t M, int64_t N, int64_t K,
-                   int64_t ld_out, int gelu, cudaStream_t st) {
-  const size_t smem = (size_t)M * f4v_row_bytes((int)((K + 63) / 64));
+static int f4_gemv(const F4Matrix& a, const F4Matrix& w, const void* bias, void* out, int64_t N, int64_t K, int gelu,
+                   cudaStream_t st) {
+  const size_t smem = f4v_smem((int)(K / 32));  // at most 36 KB: no opt-in
   const int64_t want = ((N + 127) / 128 * 32 + F4V_THREADS / 32 - 1) / (F4V_THREADS / 32);
-#define CDB_F4V(TM)                                                                                                      \
-  do {                                                                                                                   \
-    static PerDevice resident;                                                                                           \
-    const int64_t per_sm = resident.get([]() -> int64_t {                                                                \
-      return -(int64_t)cudaFuncSetAttribute(fp4_gemv_kernel<TM, NV, T>, cudaFuncAttributeMaxDynamicSharedMemorySize,     \
-                                            F4V_SMEM_LIMIT);                                                             \
-    });                                                                                                                  \
-    CDB_CUDA_CHECK((cudaError_t)(-per_sm));                                                                              \
-    const int64_t cap = (int64_t)sm_count() * 4;                                                                         \
-    CDB_CUDA_CHECK(launch_pdl(fp4_gemv_kernel<TM, NV, T>, dim3((unsigned)(want < cap ? want : cap)), dim3(F4V_THREADS), \
-                              smem, st, static_cast<const uint8_t*>(a.codes), static_cast<const uint8_t*>(a.block_scales), \
-                              a.row_scale, static_cast<const uint8_t*>(w.codes),                                         \
-                              static_cast<const uint8_t*>(w.block_scales), w.row_scale, static_cast<const T*>(bias),     \
-                              static_cast<T*>(out), ld_out, (int)N, (int)K, gelu));                                      \
-  } while (0)
-  if (M == 1) CDB_F4V(1);
-  else if (M == 2) CDB_F4V(2);
-  else if (M == 3) CDB_F4V(3);
-  else CDB_F4V(4);
-#undef CDB_F4V
+  CDB_CUDA_CHECK(launch_pdl(fp4_gemv_kernel<NV, T>, dim3((unsigned)want), dim3(F4V_THREADS), smem, st,
+                            static_cast<const uint8_t*>(a.codes), static_cast<const uint8_t*>(a.block_scales), a.row_scale,
+                            static_cast<const uint8_t*>(w.codes), static_cast<const uint8_t*>(w.block_scales), w.row_scale,
+                            static_cast<const T*>(bias), static_cast<T*>(out), (int)N, (int)K, gelu));
   return CDB_OK;
 }
 
 template <bool NV, typename T>
 static int f4_gemm(const F4Matrix& a, const F4Matrix& w, const void* bias, void* out, int64_t M, int64_t N, int64_t K,
                    int64_t ld_out, int gelu, int32_t* status_word, cudaStream_t st) {
-  if (g_f4_tile.load(std::memory_order_relaxed) == 0 && M <= F4V_MAX_M && M * f4v_row_bytes((int)((K + 63) / 64)) <= F4V_SMEM_LIMIT)
-    return f4_gemv<NV, T>(a, w, bias, out, M, N, K, ld_out, gelu, st);
+  if (g_f4_tile.load(std::memory_order_relaxed) == 0 && M == 1) return f4_gemv<NV, T>(a, w, bias, out, N, K, gelu, st);
   const F4Plan plan = f4_plan(M, N, K, sm_count());
   const int cg = plan.pair ? 2 : 1, bn = plan.bn;
   const int panels = bn > 128 ? bn / 128 : 1;
