@@ -19,7 +19,7 @@ _DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 
 
 def _rows_of(what: str, name: str, t: torch.Tensor, shape, dtype) -> torch.Tensor:
-  if tuple(t.shape) != tuple(shape) or t.dtype != dtype:
+  if t.shape != shape or t.dtype != dtype:
     raise RuntimeError(f"{what}: {name} must be {dtype} {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
   t = t if t.dim() == 3 else t.reshape(1, -1, t.shape[-1])
   return t if t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous()
@@ -28,6 +28,9 @@ def _rows_of(what: str, name: str, t: torch.Tensor, shape, dtype) -> torch.Tenso
 def _vector_of(what: str, name: str, t: Optional[torch.Tensor], batch: int, dim: int, dtype, per_batch: bool):
   if t is None:
     return None
+  if t.dtype == dtype and t.dim() == (2 if per_batch else 1) and t.shape[-1] == dim and t.stride(-1) == 1 and \
+      (not per_batch or t.shape[0] == batch):
+    return t  # the usual case: [batch, dim], or a [dim] weight
   shapes = [(dim, )] + ([(batch, dim), (1, dim)] if per_batch else [])
   if t.dtype != dtype or tuple(t.shape) not in shapes:
     raise RuntimeError(f"{what}: {name} must be {dtype} {' or '.join(map(str, shapes[:2]))}, got {t.dtype} {tuple(t.shape)}")
@@ -80,9 +83,11 @@ def gated_residual_norm(x: torch.Tensor, y: Optional[torch.Tensor] = None, gate:
   batch = x.shape[0] if x.dim() == 3 else 1
   x3 = _rows_of(what, "x", x, x.shape, x.dtype)
   y3 = None if y is None else _rows_of(what, "y", y, x.shape, x.dtype)
-  vectors = [_vector_of(what, name, t, batch, dim, x.dtype, per_batch)
-             for name, t, per_batch in (("gate", gate, True), ("post_weight", post_weight, False), ("post_bias", post_bias, False),
-                                        ("weight", weight, False), ("bias", bias, False), ("scale", scale, True), ("shift", shift, True))]
+  dtype = x.dtype
+  vectors = (_vector_of(what, "gate", gate, batch, dim, dtype, True), _vector_of(what, "post_weight", post_weight, batch, dim, dtype, False),
+             _vector_of(what, "post_bias", post_bias, batch, dim, dtype, False), _vector_of(what, "weight", weight, batch, dim, dtype, False),
+             _vector_of(what, "bias", bias, batch, dim, dtype, False), _vector_of(what, "scale", scale, batch, dim, dtype, True),
+             _vector_of(what, "shift", shift, batch, dim, dtype, True))
   x_out = x if y is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
   h = fp4 = None
   if quantize is not None:

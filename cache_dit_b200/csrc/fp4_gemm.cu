@@ -506,7 +506,7 @@ __device__ __forceinline__ float2 chunk_scales(uint32_t word, int c) {
 }
 
 template <bool NV, typename T>
-__global__ void __launch_bounds__(F4V_THREADS)
+__global__ void __launch_bounds__(F4V_THREADS, 4)
     fp4_gemv_kernel(const uint8_t* __restrict__ a_codes, const uint8_t* __restrict__ a_scales, const float* __restrict__ ra,
                     const uint8_t* __restrict__ w_codes, const uint8_t* __restrict__ w_scales, const float* __restrict__ rw,
                     const T* __restrict__ bias, T* __restrict__ out, int N, int K, int gelu) {

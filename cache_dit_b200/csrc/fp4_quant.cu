@@ -175,52 +175,82 @@ __global__ void __launch_bounds__(FP4_THREADS)
   }
 }
 
-// One unit of 16 columns per thread and step.
+// 32 bytes at p, in one store where p allows it: two of 16 bytes write every sector in two halves.
+__device__ __forceinline__ void store32(void* p, const uint32_t (&w)[8], bool whole) {
+  if (whole) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+                 "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+  } else {
+    reinterpret_cast<uint4*>(p)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    reinterpret_cast<uint4*>(p)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+  }
+}
+
+// Units of 16 columns, four per thread and step, so that four units' loads are in flight at once.
 template <typename T, bool NV>
 __global__ void __launch_bounds__(FP4_THREADS)
     fp4_dequant_rows_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
                             const float* __restrict__ row_scales, int64_t rows, int cols, T* __restrict__ out) {
   pdl_launch_dependents();
   pdl_wait_prior();
+  constexpr int AT_ONCE = 4;
   const int units = cols >> 4;
   const int64_t tiles = fp4_panel_tiles(cols, NV);
   const int64_t total = rows * units;
   const int64_t stride = (int64_t)gridDim.x * FP4_THREADS;
-  for (int64_t i = (int64_t)blockIdx.x * FP4_THREADS + threadIdx.x; i < total; i += stride) {
-    const int64_t row = total <= UINT32_MAX ? (int64_t)((uint32_t)i / (uint32_t)units) : i / units;
-    const int k = (int)(i - row * units);
-    const uint2 c = __ldcs(reinterpret_cast<const uint2*>(codes) + i);
-    const int b = NV ? k : k >> 1;
-    float step = fp4_scale_value<NV>(scales[fp4_scale_word(row, b >> 2, tiles) + (b & 3)]);
-    if (NV) step *= __ldg(row_scales + row);
-    T* dst = out + i * 16;
+  const bool whole = (reinterpret_cast<uintptr_t>(out) & 31u) == 0;
+  for (int64_t i0 = (int64_t)blockIdx.x * FP4_THREADS + threadIdx.x; i0 < total; i0 += AT_ONCE * stride) {
+    uint2 c[AT_ONCE];
+    uint32_t byte[AT_ONCE];
+    float row_scale[AT_ONCE];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      uint32_t p[4];
-      e2m1x8_to_half2(h ? c.y : c.x, p);
-      float f[8];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 v = __half22float2(*reinterpret_cast<__half2*>(&p[j]));
-        f[2 * j] = v.x * step;
-        f[2 * j + 1] = v.y * step;
+    for (int n = 0; n < AT_ONCE; ++n) {
+      const int64_t i = i0 + n * stride;
+      if (i < total) {
+        const int64_t row = total <= UINT32_MAX ? (int64_t)((uint32_t)i / (uint32_t)units) : i / units;
+        const int k = (int)(i - row * units);
+        const int b = NV ? k : k >> 1;
+        c[n] = __ldcs(reinterpret_cast<const uint2*>(codes) + i);
+        byte[n] = __ldg(scales + fp4_scale_word(row, b >> 2, tiles) + (b & 3));
+        row_scale[n] = NV ? __ldg(row_scales + row) : 1.f;
       }
-      if constexpr (sizeof(T) == 4) {
-        __stcs(reinterpret_cast<float4*>(dst) + 2 * h, make_float4(f[0], f[1], f[2], f[3]));
-        __stcs(reinterpret_cast<float4*>(dst) + 2 * h + 1, make_float4(f[4], f[5], f[6], f[7]));
-      } else {
-        uint32_t w[4];
+    }
+#pragma unroll
+    for (int n = 0; n < AT_ONCE; ++n) {
+      const int64_t i = i0 + n * stride;
+      if (i >= total) break;
+      float step = fp4_scale_value<NV>(byte[n]);
+      if (NV) step *= row_scale[n];
+      T* dst = out + i * 16;
+      uint32_t w[16];  // 16 numbers of T
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t p[4];
+        e2m1x8_to_half2(h ? c[n].y : c[n].x, p);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          if constexpr (__is_same(T, __nv_bfloat16)) {
-            const __nv_bfloat162 v = __floats2bfloat162_rn(f[2 * j], f[2 * j + 1]);
-            w[j] = *reinterpret_cast<const uint32_t*>(&v);
+          float2 v = __half22float2(*reinterpret_cast<__half2*>(&p[j]));
+          v.x *= step;
+          v.y *= step;
+          if constexpr (sizeof(T) == 4) {
+            w[h * 8 + 2 * j] = __float_as_uint(v.x);
+            w[h * 8 + 2 * j + 1] = __float_as_uint(v.y);
+          } else if constexpr (__is_same(T, __nv_bfloat16)) {
+            const __nv_bfloat162 q = __floats2bfloat162_rn(v.x, v.y);
+            w[h * 4 + j] = *reinterpret_cast<const uint32_t*>(&q);
           } else {
-            const __half2 v = __floats2half2_rn(f[2 * j], f[2 * j + 1]);
-            w[j] = *reinterpret_cast<const uint32_t*>(&v);
+            const __half2 q = __floats2half2_rn(v.x, v.y);
+            w[h * 4 + j] = *reinterpret_cast<const uint32_t*>(&q);
           }
         }
-        __stcs(reinterpret_cast<uint4*>(dst) + h, make_uint4(w[0], w[1], w[2], w[3]));
+      }
+#pragma unroll
+      for (int x = 0; x < (int)sizeof(T) / 2; ++x) {
+        uint32_t u[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) u[j] = w[x * 8 + j];
+        store32(reinterpret_cast<uint8_t*>(dst) + x * 32, u, whole);
       }
     }
   }

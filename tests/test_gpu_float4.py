@@ -198,3 +198,14 @@ def test_many_tiles_per_cta(tile, fmt):
     got = cd.float4_scaled_mm(qa, qw).double()
     assert ((got - y).abs() <= bound).all()
   assert _native.gemm_device_status(torch.device("cuda")) == 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_dequantise_into_rows_that_are_only_16_byte_aligned(dtype):
+  t = cd.float4_quantize_rows(_rows(33, 96, torch.bfloat16, 2).cuda())
+  want = cd.float4_dequantize_rows(t, dtype)
+  room = torch.full((33 * 96 + 64, ), 7.0, dtype=dtype, device="cuda")
+  off = 16 // room.element_size()
+  out = room[off:off + 33 * 96].view(33, 96)
+  _native.fp4_dequant_rows(*t._triple(), 33, 96, "nvfp4", out)
+  assert torch.equal(out, want) and (room[:off] == 7).all() and (room[off + 33 * 96:] == 7).all()
