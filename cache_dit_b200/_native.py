@@ -671,12 +671,15 @@ def gated_residual_pair(xa, gate_a, ya, xb, gate_b, yb):
 # The operators below are called for a handful of tokens too, where a kernel takes a few microseconds: their wrappers
 # pass plain integers and touch the current device only when the tensors lie on another one.
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice  # tensors of the call exist, so CUDA is initialised
 _status_ptrs = {}
 
 
 def _status_ptr(index: int) -> int:
   p = _status_ptrs.get(index)
   if p is None:
+    if index not in _mailboxes and torch.cuda.is_current_stream_capturing():
+      return None  # a mailbox made during a capture would be the graph's memory; the kernels do without
     p = _status_ptrs[index] = gemm_status_word(torch.device("cuda", index)).data_ptr()  # the mailbox is never freed
   return p
 
@@ -684,7 +687,7 @@ def _status_ptr(index: int) -> int:
 def _on_device(index: int, fn, what: str, *args):
   """fn(*args, stream) with the tensors' device current, on its current stream."""
   global launch_count
-  if index == torch.cuda.current_device():
+  if index == _current_device():
     st = fn(*args, _raw_stream(index))
   else:
     with torch.cuda.device(index):
@@ -740,7 +743,7 @@ def fp4_linear(x, ld_x: int, w, bias, out, rows: int, cols: int, fmt: str, gelu:
   index = out.device.index
   f = FP4_FORMATS[fmt]
   need = (rows * (cols >> 1) + 255) // 256 * 256 + fp4_block_scale_bytes(rows, cols, fmt) + rows * 4
-  ws = torch.empty(need, dtype=torch.uint8, device=out.device)
+  ws = out.new_empty(need, dtype=torch.uint8)
   _on_device(index, lib().cdb_fp4_linear, "cdb_fp4_linear", x.data_ptr(), ld_x, ctypes.byref(Fp4Matrix(*map(_dp, w))), _dp(bias),
              out.data_ptr(), rows, n, cols, n, f, DTYPE_ID[out.dtype], int(gelu), ws.data_ptr(), need, _status_ptr(index))
 
@@ -788,7 +791,7 @@ class Heads(ctypes.Structure):
 
 
 def _workspace_bytes_on(index: int, *args) -> int:
-  if index == torch.cuda.current_device():
+  if index == _current_device():
     return lib().cdb_cross_attention_workspace_bytes(*args)
   with torch.cuda.device(index):
     return lib().cdb_cross_attention_workspace_bytes(*args)
@@ -801,7 +804,7 @@ def cross_attention(q, k, v, key_mask, scale: float, out):
   skv, kv_h = k.shape[1], k.shape[2]
   index = q.device.index
   need = _workspace_bytes_on(index, b, sq, skv, h, kv_h, d, int(key_mask is not None))
-  ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+  ws = q.new_empty(need, dtype=torch.uint8) if need else None
   qh, kh, vh = (Heads(t.data_ptr(), *t.stride()[:3]) for t in (q, k, v))
   _on_device(index, lib().cdb_cross_attention, "cdb_cross_attention", ctypes.byref(qh), ctypes.byref(kh), ctypes.byref(vh),
              _dp(key_mask), 0 if key_mask is None else key_mask.stride(0), out.data_ptr(), b, sq, skv, h, kv_h, d, scale,

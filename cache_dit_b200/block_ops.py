@@ -88,7 +88,7 @@ def gated_residual_norm(x: torch.Tensor, y: Optional[torch.Tensor] = None, gate:
              _vector_of(what, "post_bias", post_bias, batch, dim, dtype, False), _vector_of(what, "weight", weight, batch, dim, dtype, False),
              _vector_of(what, "bias", bias, batch, dim, dtype, False), _vector_of(what, "scale", scale, batch, dim, dtype, True),
              _vector_of(what, "shift", shift, batch, dim, dtype, True))
-  x_out = x if y is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+  x_out = x if y is None else x.new_empty(x.shape)
   h = fp4 = None
   if quantize is not None:
     h4 = empty_rows(x.shape[:-1], dim, quantize, x.device)
@@ -96,7 +96,7 @@ def gated_residual_norm(x: torch.Tensor, y: Optional[torch.Tensor] = None, gate:
     aligned = lambda t: t is None or (t.data_ptr() % 16 == 0 and all(s * t.element_size() % 16 == 0 for s in t.stride()[:-1]))
     x3, y3, *vectors = (t if aligned(t) else t.clone(memory_format=torch.contiguous_format) for t in (x3, y3, *vectors))
   elif norm is not None:
-    h = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    h = x.new_empty(x.shape)
   if x.numel():
     _native.gated_residual_norm(x3, y3, *vectors, x_out, h, fp4, post_norm, norm, float(residual_scale), float(post_eps), float(eps))
   return x_out, h if quantize is None else h4
@@ -137,7 +137,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, key_mask:
   if not (scale > 0.0 and math.isfinite(scale)):
     raise RuntimeError(f"{what}: scale must be positive and finite, got {scale}")
   refuse(what, q, k, v, key_mask)
-  out = torch.empty((b, sq, h, d), dtype=q.dtype, device=q.device)
+  out = q.new_empty((b, sq, h, d))
   if out.numel() == 0:
     return out
   if skv == 0:

@@ -285,7 +285,7 @@ __global__ void __launch_bounds__(XA_THREADS, 1) cross_attention_kernel(const __
   } else if (warp >= XA_MMA_WARP) {
     // ---------------- products of tile t ----------------
     // For every step: S = Q_t K^T, then O_t += P_t V of the step before, whose exponentials ran meanwhile.  A warp per
-    // tile: a satisfied wait takes a hundred clocks, and one warp that did them all for both tiles set the pace.
+    // tile: a satisfied wait takes 60 to 100 clocks, and one warp that did them all for both tiles set the pace.
     const int t = warp - XA_MMA_WARP;
     constexpr uint32_t idesc_s = xa_idesc(BF16, XA_KEYS, false);
     constexpr uint32_t idesc_o = xa_idesc(BF16, DP, true);

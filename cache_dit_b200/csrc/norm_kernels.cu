@@ -50,8 +50,15 @@ __device__ __forceinline__ void unpack8(const uint4& v, float (&f)[8]) {
     }
   }
 }
-// Eight consecutive elements; `n` of them exist (the rest read as 0 and are not written).
-template <typename T, bool ALIGNED>
+// Which eight elements of a row pack `i` of thread `t` is: eight in a row, as 16-byte accesses, where rows allow it; else
+// TPR apart, so that neighbouring threads still touch neighbouring elements (eight in a row, one by one: 154 us for
+// 30000 x 1001 bf16).
+template <int TPR, bool ALIGNED>
+__device__ __forceinline__ int first_column(int t, int i) {
+  return ALIGNED ? (t + i * TPR) * 8 : i * 8 * TPR + t;
+}
+// The eight elements from p on; `n` columns are left in the row (what is beyond reads as 0 and is not written).
+template <typename T, bool ALIGNED, int TPR>
 __device__ __forceinline__ void load8(const T* p, int n, float (&f)[8]) {
   if constexpr (ALIGNED) {
     if constexpr (sizeof(T) == 4) {
@@ -62,10 +69,10 @@ __device__ __forceinline__ void load8(const T* p, int n, float (&f)[8]) {
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = i < n ? to_f(p[i]) : 0.f;
+    for (int i = 0; i < 8; ++i) f[i] = i * TPR < n ? to_f(p[i * TPR]) : 0.f;
   }
 }
-template <typename T, bool ALIGNED>
+template <typename T, bool ALIGNED, int TPR>
 __device__ __forceinline__ void store8(T* p, int n, const float (&f)[8]) {
   if constexpr (ALIGNED) {
     if constexpr (sizeof(T) == 4) {
@@ -88,7 +95,7 @@ __device__ __forceinline__ void store8(T* p, int n, const float (&f)[8]) {
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (i < n) p[i] = from_f<T>(f[i]);
+      if (i * TPR < n) p[i * TPR] = from_f<T>(f[i]);
   }
 }
 
@@ -187,12 +194,12 @@ __device__ __forceinline__ float normalise(float (&v)[PACKS][8], int kind, int t
     fill8(minus, -mean);
 #pragma unroll
     for (int i = 0; i < PACKS; ++i) {
-      const int left = dim - (t + i * TPR) * 8;
+      const int left = dim - first_column<TPR, ALIGNED>(t, i);
       if constexpr (ALIGNED) {  // a pack is all there or not at all
         if (left > 0) add8(v[i], v[i], minus);
       } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[i][j] = j < left ? v[i][j] - mean : 0.f;
+        for (int j = 0; j < 8; ++j) v[i][j] = j * TPR < left ? v[i][j] - mean : 0.f;
       }
     }
   }
@@ -272,11 +279,11 @@ __global__ void __launch_bounds__(NORM_THREADS) gated_residual_norm_kernel(const
     float v[PACKS][8];
 #pragma unroll
     for (int i = 0; i < PACKS; ++i) {
-      const int c = (t + i * TPR) * 8;
+      const int c = first_column<TPR, ALIGNED>(t, i);
       if constexpr (AHEAD) {
         unpack8<T>(ax[i], v[i]);
       } else if (c < dim) {
-        load8<T, ALIGNED>(xr + c, dim - c, v[i]);
+        load8<T, ALIGNED, TPR>(xr + c, dim - c, v[i]);
       } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
@@ -289,21 +296,21 @@ __global__ void __launch_bounds__(NORM_THREADS) gated_residual_norm_kernel(const
         float f[8], alpha[8];
         fill8(alpha, a.residual_scale);
         if (gate != nullptr) {
-          load8<T, ALIGNED>(gate + b * a.gate_batch + c, dim - c, f);
+          load8<T, ALIGNED, TPR>(gate + b * a.gate_batch + c, dim - c, f);
           mul8(f, f, alpha);
           fma8(v[i], f, y, v[i]);
         } else {
           fma8(v[i], alpha, y, v[i]);
         }
-        store8<T, ALIGNED>(xo + c, dim - c, v[i]);
+        store8<T, ALIGNED, TPR>(xo + c, dim - c, v[i]);
       };
       if constexpr (POST) {
         float y[PACKS][8];
 #pragma unroll
         for (int i = 0; i < PACKS; ++i) {
-          const int c = (t + i * TPR) * 8;
+          const int c = first_column<TPR, ALIGNED>(t, i);
           if (c < dim) {
-            load8<T, ALIGNED>(yr + c, dim - c, y[i]);
+            load8<T, ALIGNED, TPR>(yr + c, dim - c, y[i]);
           } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j) y[i][j] = 0.f;
@@ -312,17 +319,17 @@ __global__ void __launch_bounds__(NORM_THREADS) gated_residual_norm_kernel(const
         const float r = normalise<TPR, PACKS, ALIGNED>(y, a.post, t, dim, a.post_eps, s_words[parity]);
 #pragma unroll
         for (int i = 0; i < PACKS; ++i) {
-          const int c = (t + i * TPR) * 8;
+          const int c = first_column<TPR, ALIGNED>(t, i);
           if (c < dim) {
             float f[8];
             float g[8];
             fill8(f, r);
             if (post_weight != nullptr) {
-              load8<T, ALIGNED>(post_weight + c, dim - c, g);
+              load8<T, ALIGNED, TPR>(post_weight + c, dim - c, g);
               mul8(f, f, g);
             }
             fill8(g, 0.f);
-            if (post_bias != nullptr) load8<T, ALIGNED>(post_bias + c, dim - c, g);
+            if (post_bias != nullptr) load8<T, ALIGNED, TPR>(post_bias + c, dim - c, g);
             fma8(y[i], y[i], f, g);
             add(i, c, y[i]);
           }
@@ -330,11 +337,11 @@ __global__ void __launch_bounds__(NORM_THREADS) gated_residual_norm_kernel(const
       } else {
 #pragma unroll
         for (int i = 0; i < PACKS; ++i) {
-          const int c = (t + i * TPR) * 8;
+          const int c = first_column<TPR, ALIGNED>(t, i);
           if (c < dim) {
             float y[8];
             if constexpr (AHEAD) unpack8<T>(ay[i], y);
-            else load8<T, ALIGNED>(yr + c, dim - c, y);
+            else load8<T, ALIGNED, TPR>(yr + c, dim - c, y);
             add(i, c, y);
           }
         }
@@ -346,28 +353,28 @@ __global__ void __launch_bounds__(NORM_THREADS) gated_residual_norm_kernel(const
     uint32_t top[PACKS];
 #pragma unroll
     for (int i = 0; i < PACKS; ++i) {
-      const int c = (t + i * TPR) * 8;
+      const int c = first_column<TPR, ALIGNED>(t, i);
       top[i] = 0u;
       if (c < dim) {
         float f[8], g[8];
         fill8(f, r);
         if (weight != nullptr) {
-          load8<T, ALIGNED>(weight + c, dim - c, g);
+          load8<T, ALIGNED, TPR>(weight + c, dim - c, g);
           mul8(f, f, g);
         }
         fill8(g, 0.f);
-        if (bias != nullptr) load8<T, ALIGNED>(bias + c, dim - c, g);
+        if (bias != nullptr) load8<T, ALIGNED, TPR>(bias + c, dim - c, g);
         fma8(v[i], v[i], f, g);
         if (a.scale != nullptr) {
-          load8<T, ALIGNED>(static_cast<const T*>(a.scale) + b * a.scale_batch + c, dim - c, f);
-          load8<T, ALIGNED>(static_cast<const T*>(a.shift) + b * a.shift_batch + c, dim - c, g);
+          load8<T, ALIGNED, TPR>(static_cast<const T*>(a.scale) + b * a.scale_batch + c, dim - c, f);
+          load8<T, ALIGNED, TPR>(static_cast<const T*>(a.shift) + b * a.shift_batch + c, dim - c, g);
           float one[8];
           fill8(one, 1.f);
           add8(f, f, one);
           fma8(v[i], v[i], f, g);
         }
         if (!quantise) {
-          store8<T, ALIGNED>(static_cast<T*>(a.h_out) + row * dim + c, dim - c, v[i]);
+          store8<T, ALIGNED, TPR>(static_cast<T*>(a.h_out) + row * dim + c, dim - c, v[i]);
         } else {
           top[i] = round8<T>(v[i]);
         }
@@ -420,7 +427,8 @@ static int launch_norm(const NormArgs& a, cudaStream_t st) {
   return CDB_OK;
 }
 
-// Threads per row: the fewest that hold it in at most six packs of 8 elements (64 fp32 registers for the widest rows).
+// Threads per row: the fewest that hold it in four or five packs of 8 elements, up to eight for the widest rows (64 fp32
+// registers).
 template <typename T>
 static int dispatch_norm(const NormArgs& a, bool aligned, cudaStream_t st) {
   // with 4-bit output the padded block scales need a thread each

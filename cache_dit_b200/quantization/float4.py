@@ -25,7 +25,7 @@ _DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 _OUT_DTYPES = (torch.bfloat16, torch.float16)
 
 
-@dataclasses.dataclass(frozen=True)
+@dataclasses.dataclass(frozen=True, eq=False)
 class Float4Rows:
   """A [..., cols] matrix in 4 bits: codes uint8 [..., cols / 2] (even column in the low half), the tiled block scales
   (uint8, flat), and for nvfp4 one float32 per row."""
@@ -210,7 +210,7 @@ def float4_linear(x: torch.Tensor, w: Float4Rows, bias: Optional[torch.Tensor] =
   if cols != w.cols:
     raise RuntimeError(f"{what}: x has {cols} columns, the weight {w.cols}")
   refuse(what, x, w.codes, w.block_scales, w.row_scale, bias)
-  out = torch.empty((*x.shape[:-1], n), dtype=x.dtype, device=x.device)
+  out = x.new_empty((*x.shape[:-1], n))
   if rows:
     x2, ld = _as_matrix(x, rows, cols)
     _native.fp4_linear(x2, ld, _aligned(w)._triple(), bias, out, rows, cols, w.format, gelu)

@@ -145,6 +145,19 @@ def test_four_bit_linears_are_selected_by_their_own_shapes(monkeypatch):
   assert seen == [((32, 64), "mxfp4")]  # 48 columns are no whole block of 32, 20 rows no multiple of 8
 
 
+def test_encoder_attention_with_a_prompt_mask_on_cpu():
+  from cache_dit_b200.synthetic.layers import encoder_attention
+  g = torch.Generator().manual_seed(0)
+  q, k, v = (torch.randn(3, n, 2, 16, generator=g) for n in (5, 7, 7))
+  mask = torch.arange(7)[None] < torch.tensor([7, 3, 0])[:, None]
+  v[~mask] = float("nan")
+  got = encoder_attention(q, k, v, mask)
+  for i, n in ((0, 7), (1, 3)):
+    alone = encoder_attention(q[i:i + 1], k[i:i + 1, :n], v[i:i + 1, :n])
+    assert torch.allclose(got[i], alone[0], atol=1e-6)
+  assert (got[2] == 0).all()
+
+
 def test_latched_codes_name_the_operator():
   for code, name in ((24, "4-bit product"), (36, "cross attention"), (13, "FP8 GEMM")):
     with pytest.raises(nat.DeviceTimeoutError, match=name):
