@@ -14,8 +14,9 @@
 //     the next tile's MMAs wait for is that read.
 //   * one row: no tile; the weights are streamed once by the CUDA cores (fp4_gemv_kernel).
 //
-// Warp roles (224 threads): warp 0 = TMA producer, warp 1 = tensor memory owner and MMA issuer, warps 2..5 = epilogue,
-// warp 6 = block scales to tensor memory.
+// Warp roles (352 threads): warp 0 = TMA producer, warp 1 = tensor memory owner and MMA issuer, warps 2..9 = epilogue (two
+// per 32 rows, half of the columns each: the last tile's epilogue has nothing to hide under), warp 10 = block scales to
+// tensor memory.
 // Every wait is bounded (bounded_wait): on expiry the roles drain, tensor memory is freed and the kernel returns.
 #include <cuda_fp16.h>
 
@@ -27,10 +28,10 @@
 
 namespace cdb {
 
-constexpr int F4_THREADS = 224;
+constexpr int F4_THREADS = 352;
 constexpr int F4_EPI_WARP0 = 2;
-constexpr int F4_EPI_THREADS = 128;
-constexpr int F4_SCALE_WARP = 6;
+constexpr int F4_EPI_THREADS = 256;
+constexpr int F4_SCALE_WARP = 10;
 constexpr int F4_MAX_STAGES = 8;
 constexpr int F4_MAX_SLOTS = 8;
 constexpr int F4_MAX_BN = 256;
@@ -38,7 +39,7 @@ constexpr int F4_A_BYTES = 128 * 128;     // 128 rows of one step's codes
 constexpr uint32_t F4_TMEM_COLS = 512;
 constexpr uint32_t F4_SHARED_COL = 160;   // where the second accumulator starts when bn = 256
 constexpr int F4_BLOCK_BYTES = 32 * 64 * 2;                      // one staged block of output: 32 rows x 64 columns
-constexpr int F4_STAGING_BYTES = (F4_EPI_THREADS / 32) * 2 * F4_BLOCK_BYTES;
+constexpr int F4_STAGING_BYTES = (F4_EPI_THREADS / 32) * F4_BLOCK_BYTES;
 constexpr int F4_SMEM_LIMIT = 232448;
 
 struct __align__(8) F4Barriers {
@@ -172,12 +173,11 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 
 // One staged block: 32 rows x 64 columns starting at local column `c0` of the tile, from 2 x 32 accumulator registers.
 template <typename T>
-__device__ __forceinline__ void f4_store_block(const F4Params& p, uint8_t* staging, uint32_t& blocks_done,
+__device__ __forceinline__ void f4_store_block(const F4Params& p, uint8_t* block,
                                                const uint32_t (&lo)[32], const uint32_t (&hi)[32], int c0, int n0,
                                                int row0, float rs, const float2* s_col, int lane) {
   if (n0 + c0 >= p.N) return;
-  uint8_t* block = staging + (blocks_done & 1u) * F4_BLOCK_BYTES;
-  if (lane == 0) bulk_wait_group_read<1>();  // the store that used this block two blocks ago is done reading
+  if (lane == 0) bulk_wait_group_read<0>();  // the store before this one is done reading
   __syncwarp();
   uint8_t* rowp = block + lane * 128;
 #pragma unroll
@@ -204,7 +204,6 @@ __device__ __forceinline__ void f4_store_block(const F4Params& p, uint8_t* stagi
     tma_store_2d(&p.map_out, block, n0 + c0, row0);
     bulk_commit_group();
   }
-  ++blocks_done;
 }
 
 template <int CG, int BN, bool NV, typename T>
@@ -392,9 +391,10 @@ __global__ void __launch_bounds__(F4_THREADS, 1) fp4_gemm_kernel(const __grid_co
     // ---------------- epilogue: this CTA's 128 rows x bn columns ----------------
     const int quarter = warp & 3;
     const int et = threadIdx.x - F4_EPI_WARP0 * 32;
-    uint8_t* staging = s_staging + quarter * 2 * F4_BLOCK_BYTES;
+    const int half = (warp - F4_EPI_WARP0) >> 2;  // of the tile's columns
+    uint8_t* staging = s_staging + (warp - F4_EPI_WARP0) * F4_BLOCK_BYTES;
     const T* bias = static_cast<const T*>(p.bias);
-    uint32_t n_tile = 0, blocks_done = 0;
+    uint32_t n_tile = 0;
     bool ok = true;
     for (int tile = first; tile < p.num_tiles && ok; tile += step, ++n_tile) {
       int mi, ni;
@@ -413,7 +413,7 @@ __global__ void __launch_bounds__(F4_THREADS, 1) fp4_gemm_kernel(const __grid_co
         s_col[c] = v;
       }
       ok = bounded_wait(&gb->acc_full[buf], (n_tile >> 1) & 1u, &gb->abort_flag, status_word, 25);
-      ok = f4_epi_all(ok);  // publishes s_col, and makes the decision to go on the same in all four warps
+      ok = f4_epi_all(ok);  // publishes s_col, and makes the decision to go on the same in all its warps
       if (!ok) break;
       tcgen05_fence_after();
       const int row = row0 + lane;
@@ -435,35 +435,40 @@ __global__ void __launch_bounds__(F4_THREADS, 1) fp4_gemm_kernel(const __grid_co
           tmem_ld_32x32b_x32(taddr + c, lo);
           tmem_ld_32x32b_x32(taddr + c + 32, hi);
           tmem_ld_wait();
-          f4_store_block<T>(p, staging, blocks_done, lo, hi, c, n0, row0, rs, s_col, lane);
+          f4_store_block<T>(p, staging, lo, hi, c, n0, row0, rs, s_col, lane);
         }
       };
       if constexpr (!shared_acc) {
-        if (live) plain_blocks(0, bn);
+        constexpr int split = bn > 64 ? bn / 2 : 64;
+        if (live) plain_blocks(half ? split : 0, half ? bn : split);
         release();
       } else if (!live) {
         release();
       } else {
-        // the columns that the other accumulator overlaps: 160..255 of the first, 0..95 of the second
-        uint32_t s0[32], s1[32], s2[32], x[32];
-        const uint32_t at = taddr + (buf == 0 ? F4_SHARED_COL : 0u);
-        tmem_ld_32x32b_x32(at, s0);
-        tmem_ld_32x32b_x32(at + 32, s1);
-        tmem_ld_32x32b_x32(at + 64, s2);
-        tmem_ld_wait();
-        release();
-        if (buf == 0) {
-          f4_store_block<T>(p, staging, blocks_done, s1, s2, 192, n0, row0, rs, s_col, lane);
-          tmem_ld_32x32b_x32(taddr + 128, x);
-          tmem_ld_wait();
-          f4_store_block<T>(p, staging, blocks_done, x, s0, 128, n0, row0, rs, s_col, lane);
-          plain_blocks(0, 128);
+        // The columns that the other accumulator overlaps are 160..255 of the first and 0..95 of the second: all of them in
+        // one half.
+        if ((int)buf == half) {
+          release();
+          plain_blocks(half * 128, half * 128 + 128);
         } else {
-          f4_store_block<T>(p, staging, blocks_done, s0, s1, 0, n0, row0, rs, s_col, lane);
-          tmem_ld_32x32b_x32(taddr + 96, x);
+          uint32_t s0[32], s1[32], s2[32], x[32];
+          const uint32_t at = taddr + (buf == 0 ? F4_SHARED_COL : 0u);
+          tmem_ld_32x32b_x32(at, s0);
+          tmem_ld_32x32b_x32(at + 32, s1);
+          tmem_ld_32x32b_x32(at + 64, s2);
           tmem_ld_wait();
-          f4_store_block<T>(p, staging, blocks_done, s2, x, 64, n0, row0, rs, s_col, lane);
-          plain_blocks(128, 256);
+          release();
+          if (buf == 0) {
+            f4_store_block<T>(p, staging, s1, s2, 192, n0, row0, rs, s_col, lane);
+            tmem_ld_32x32b_x32(taddr + 128, x);
+            tmem_ld_wait();
+            f4_store_block<T>(p, staging, x, s0, 128, n0, row0, rs, s_col, lane);
+          } else {
+            f4_store_block<T>(p, staging, s0, s1, 0, n0, row0, rs, s_col, lane);
+            tmem_ld_32x32b_x32(taddr + 96, x);
+            tmem_ld_wait();
+            f4_store_block<T>(p, staging, s2, x, 64, n0, row0, rs, s_col, lane);
+          }
         }
         tcgen05_fence_before();  // orders these reads before the next barrier, behind which MMAs may overwrite them
       }
