@@ -15,7 +15,7 @@
 //     step of both tiles; the tensor core needs 2040.)  At d > 64 there is room for one S, which the tiles take in turn;
 //   * the output goes through shared memory and TMA: stores of a thread per row took 5500 clocks a tile;
 //   * O is rescaled only when a row's maximum has grown by more than 2^8: until then P simply grows to at most 2^8, which
-//     costs nothing in a floating type.  P is rounded to 16 bits for the product (a relative 2^-9 or 2^-12 each,
+//     costs nothing in a floating type.  P is rounded to 16 bits for the product (a relative 2^-8 or 2^-11 each at most,
 //     averaged over the keys); m, l, S and O are fp32.
 // Few rows over many keys: the key range is split over CTAs, partial (O, m, l) are joined by a second kernel.
 //
