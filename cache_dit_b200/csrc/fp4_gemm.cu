@@ -627,11 +627,11 @@ static std::atomic<int> g_f4_tile{0};
 // Tile shape of a launch, by a cost in steps of a 256-column pair tile (0.55 us): waves of tiles x steps x what a step
 // of that shape costs, plus what a launch of it costs whatever K (filling the ring, the last tile's epilogue).  Fitted
 // to nvfp4 launches with cold weights (M, N, K: 4608 x 5120 x 13824, 1153 x 12288 x 5120, 512 x 13824 x 5120, 77 x 5120
-// x 4096): pair 256 / pair 128 / single 128 / single 64 take 147 / 241 / 239 / 427, 51 / 59 / 60 / 105,
-// 30.2 / 29.2 / 29.4 / 51 and 16.1 / 12.1 / 11.3 / 10.7 us.
+// x 4096): pair 256 / pair 128 / single 128 / single 64 take 141 / 213 / 211 / 417, 49 / 61 / 59 / 104,
+// 27.7 / 29.4 / 28.6 / 51 and 13.8 / 11.0 / 10.2 / 10.0 us.
 static F4Plan f4_plan(int64_t M, int64_t N, int64_t K, int sms) {
   const struct { bool pair; int bn; double step, launch; } shapes[] = {
-      {true, 256, 1.0, 15.0}, {true, 128, 0.82, 6.0}, {false, 128, 0.81, 5.5}, {false, 64, 0.72, 6.0}};
+      {true, 256, 1.0, 9.0}, {true, 128, 0.82, 6.0}, {false, 128, 0.81, 5.5}, {false, 64, 0.72, 6.0}};
   const int64_t k_steps = (K + FP4_STEP_COLS - 1) / FP4_STEP_COLS;
   const int forced = g_f4_tile.load(std::memory_order_relaxed);
   if (forced != 0) return F4Plan{forced < 0, forced < 0 ? -forced : forced};
