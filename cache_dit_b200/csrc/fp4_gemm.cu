@@ -493,6 +493,8 @@ __global__ void __launch_bounds__(F4_THREADS, 1) fp4_gemm_kernel(const __grid_co
 // bytes of codes of each, one 16-byte load of scales, and the activations, from shared memory, once for all four.  The
 // products of a block of 16 are multiples of 0.25 and at most 36: eight of them sum exactly in f16 (at most 288), so the two
 // halves of a packed f16 accumulator hold the sum exactly; blocks are summed in fp32.
+// Where the columns are too few to fill the SMs with warps, `split` warps of a block share their columns and take every
+// split-th 32 chunks of K each; their sums are added in order.
 // From two rows on the tile kernels are faster (4 x 30720 x 5120: 29 us against 50 us of this kernel with four rows).
 constexpr int F4V_THREADS = 256;
 __host__ __device__ constexpr size_t f4v_smem(int chunks) { return (size_t)chunks * (64 + 8); }  // f16 codes, two fp32 scales
@@ -514,7 +516,7 @@ template <bool NV, typename T>
 __global__ void __launch_bounds__(F4V_THREADS, 4)
     fp4_gemv_kernel(const uint8_t* __restrict__ a_codes, const uint8_t* __restrict__ a_scales, const float* __restrict__ ra,
                     const uint8_t* __restrict__ w_codes, const uint8_t* __restrict__ w_scales, const float* __restrict__ rw,
-                    const T* __restrict__ bias, T* __restrict__ out, int N, int K, int gelu) {
+                    const T* __restrict__ bias, T* __restrict__ out, int N, int K, int split, int gelu) {
   pdl_launch_dependents();
   pdl_wait_prior();
   extern __shared__ __align__(16) uint8_t smem_raw[];
@@ -535,62 +537,73 @@ __global__ void __launch_bounds__(F4V_THREADS, 4)
     s_s[c] = chunk_scales<NV>(*reinterpret_cast<const uint32_t*>(a_scales + fp4_scale_word(0, c >> PER_WORD, tiles)), c);
   }
   __syncthreads();
-  const int lane = threadIdx.x & 31;
-  const int warp = (blockIdx.x * F4V_THREADS + threadIdx.x) >> 5;
-  const int nwarps = (gridDim.x * F4V_THREADS) >> 5;
-  const int groups = ((N + 127) >> 7) * 32;
-  for (int g = warp; g < groups; g += nwarps) {
-    const int n0 = (g >> 5) * 128 + (g & 31);
-    const uint4* wrow[4];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int part = warp & (split - 1);
+  const int g = blockIdx.x * (F4V_THREADS / 32 / split) + warp / split;
+  // g < groups for every warp: the groups, a multiple of 32, are a whole number of blocks.
+  const int n0 = (g >> 5) * 128 + (g & 31);
+  const uint4* wrow[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) wrow[j] = reinterpret_cast<const uint4*>(w_codes + (int64_t)min(n0 + 32 * j, N - 1) * (K >> 1));
-    const uint8_t* srow = w_scales + fp4_scale_word(n0, 0, tiles);
-    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int j = 0; j < 4; ++j) wrow[j] = reinterpret_cast<const uint4*>(w_codes + (int64_t)min(n0 + 32 * j, N - 1) * (K >> 1));
+  const uint8_t* srow = w_scales + fp4_scale_word(n0, 0, tiles);
+  float acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 2
-    for (int c = lane; c < chunks; c += 32) {
-      const uint4 sw = __ldg(reinterpret_cast<const uint4*>(srow + (c >> PER_WORD) * 512));
-      uint4 wv[4];
+  for (int c = part * 32 + lane; c < chunks; c += 32 * split) {
+    const uint4 sw = __ldg(reinterpret_cast<const uint4*>(srow + (c >> PER_WORD) * 512));
+    uint4 wv[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) wv[j] = __ldcs(wrow[j] + c);
-      const float2 as = s_s[c];
-      uint4 av[4];
+    for (int j = 0; j < 4; ++j) wv[j] = __ldcs(wrow[j] + c);
+    const float2 as = s_s[c];
+    uint4 av[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) av[j] = s_a[j * chunks + c];
-      const uint32_t sword[4] = {sw.x, sw.y, sw.z, sw.w};
-      auto h2 = [](const uint32_t& u) { return *reinterpret_cast<const __half2*>(&u); };
+    for (int j = 0; j < 4; ++j) av[j] = s_a[j * chunks + c];
+    const uint32_t sword[4] = {sw.x, sw.y, sw.z, sw.w};
+    auto h2 = [](const uint32_t& u) { return *reinterpret_cast<const __half2*>(&u); };
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 ws = chunk_scales<NV>(sword[j], c);
-        const uint32_t word[4] = {wv[j].x, wv[j].y, wv[j].z, wv[j].w};
+    for (int j = 0; j < 4; ++j) {
+      const float2 ws = chunk_scales<NV>(sword[j], c);
+      const uint32_t word[4] = {wv[j].x, wv[j].y, wv[j].z, wv[j].w};
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          uint32_t f0[4], f1[4];
-          e2m1x8_to_half2(word[2 * b], f0);
-          e2m1x8_to_half2(word[2 * b + 1], f1);
-          __half2 t = __hmul2(h2(f0[0]), h2(av[2 * b].x));
-          t = __hfma2(h2(f0[1]), h2(av[2 * b].y), t);
-          t = __hfma2(h2(f0[2]), h2(av[2 * b].z), t);
-          t = __hfma2(h2(f0[3]), h2(av[2 * b].w), t);
-          t = __hfma2(h2(f1[0]), h2(av[2 * b + 1].x), t);
-          t = __hfma2(h2(f1[1]), h2(av[2 * b + 1].y), t);
-          t = __hfma2(h2(f1[2]), h2(av[2 * b + 1].z), t);
-          t = __hfma2(h2(f1[3]), h2(av[2 * b + 1].w), t);
-          const float2 d = __half22float2(t);
-          acc[j] = fmaf(d.x + d.y, b ? ws.y * as.y : ws.x * as.x, acc[j]);
-        }
+      for (int b = 0; b < 2; ++b) {
+        uint32_t f0[4], f1[4];
+        e2m1x8_to_half2(word[2 * b], f0);
+        e2m1x8_to_half2(word[2 * b + 1], f1);
+        __half2 t = __hmul2(h2(f0[0]), h2(av[2 * b].x));
+        t = __hfma2(h2(f0[1]), h2(av[2 * b].y), t);
+        t = __hfma2(h2(f0[2]), h2(av[2 * b].z), t);
+        t = __hfma2(h2(f0[3]), h2(av[2 * b].w), t);
+        t = __hfma2(h2(f1[0]), h2(av[2 * b + 1].x), t);
+        t = __hfma2(h2(f1[1]), h2(av[2 * b + 1].y), t);
+        t = __hfma2(h2(f1[2]), h2(av[2 * b + 1].z), t);
+        t = __hfma2(h2(f1[3]), h2(av[2 * b + 1].w), t);
+        const float2 d = __half22float2(t);
+        acc[j] = fmaf(d.x + d.y, b ? ws.y * as.y : ws.x * as.x, acc[j]);
       }
     }
+  }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc[j] = warp_sum(acc[j]);
+  for (int j = 0; j < 4; ++j) acc[j] = warp_sum(acc[j]);
+  if (split > 1) {
+    __shared__ float4 s_part[F4V_THREADS / 32];
+    if (lane == 0) s_part[warp] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+    __syncthreads();
+    if (part != 0) return;
+    for (int i = 1; i < split; ++i) {
+      const float4 more = s_part[warp + i];
+      acc[0] += more.x;
+      acc[1] += more.y;
+      acc[2] += more.z;
+      acc[3] += more.w;
+    }
+  }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {  // lane j writes column j
-      const int n = n0 + 32 * j;
-      if (lane == j && n < N) {
-        const float cs = rw != nullptr ? __ldg(rw + n) : 1.f;
-        float v = fmaf(acc[j] * (ra != nullptr ? __ldg(ra) : 1.f), cs, bias != nullptr ? (float)bias[n] : 0.f);
-        if (gelu) v = gelu_tanh(v);
-        out[n] = (T)v;
-      }
+  for (int j = 0; j < 4; ++j) {  // lane j writes column j
+    const int n = n0 + 32 * j;
+    if (lane == j && n < N) {
+      const float cs = rw != nullptr ? __ldg(rw + n) : 1.f;
+      float v = fmaf(acc[j] * (ra != nullptr ? __ldg(ra) : 1.f), cs, bias != nullptr ? (float)bias[n] : 0.f);
+      if (gelu) v = gelu_tanh(v);
+      out[n] = (T)v;
     }
   }
 }
@@ -675,11 +688,15 @@ template <bool NV, typename T>
 static int f4_gemv(const F4Matrix& a, const F4Matrix& w, const void* bias, void* out, int64_t N, int64_t K, int gelu,
                    cudaStream_t st) {
   const size_t smem = f4v_smem((int)(K / 32));  // at most 36 KB: no opt-in
-  const int64_t want = ((N + 127) / 128 * 32 + F4V_THREADS / 32 - 1) / (F4V_THREADS / 32);
+  // Four blocks an SM are resident: split K until there are as many, down to one load per lane.
+  const int64_t warps = (N + 127) / 128 * 32;
+  int split = 1;
+  while (split < F4V_THREADS / 32 && warps * split < (int64_t)sm_count() * 4 * (F4V_THREADS / 32) && split * 64 <= K / 32) split *= 2;
+  const int64_t want = warps * split / (F4V_THREADS / 32);  // warps is a multiple of 32: no rest
   CDB_CUDA_CHECK(launch_pdl(fp4_gemv_kernel<NV, T>, dim3((unsigned)want), dim3(F4V_THREADS), smem, st,
                             static_cast<const uint8_t*>(a.codes), static_cast<const uint8_t*>(a.block_scales), a.row_scale,
                             static_cast<const uint8_t*>(w.codes), static_cast<const uint8_t*>(w.block_scales), w.row_scale,
-                            static_cast<const T*>(bias), static_cast<T*>(out), (int)N, (int)K, gelu));
+                            static_cast<const T*>(bias), static_cast<T*>(out), (int)N, (int)K, split, gelu));
   return CDB_OK;
 }
 

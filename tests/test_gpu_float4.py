@@ -141,6 +141,17 @@ def test_product(m, n, k, fmt):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("n,k", [(8, 2016), (8, 2048), (136, 4096), (264, 8224), (1000, 16384), (4744, 1056), (9480, 2080), (19000, 544)])
+def test_product_of_one_row(n, k, fmt):
+  """Few columns split K over the warps of a block, many do not; K ends inside a warp's share."""
+  qa, qw, va, vw = _operands(1, n, k, fmt, n + k)
+  y = va @ vw.T
+  got = cd.float4_scaled_mm(qa, qw)
+  assert torch.equal(got, cd.float4_scaled_mm(qa, qw))
+  assert (np.abs(got.double().cpu().numpy() - y) <= _product_bound(va, vw, y, k, torch.bfloat16)).all()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("m,n,k,gelu", [(1, 72, 96, True), (4, 256, 512, False), (60, 320, 512, True), (700, 1288, 1024, True),
                                         (700, 1288, 1024, False)])
