@@ -274,12 +274,14 @@ __global__ void __launch_bounds__(XA_THREADS, 1) cross_attention_kernel(const __
           }
         }
       }
-      // Copies in flight land (bounded, also after an abort) before the CTA retires: the last use of every barrier.
+      // The CTA may not retire while copies into its shared memory are in flight, while MMAs read it or while a commit has
+      // yet to arrive on one of its barriers: wait (bounded, also after an abort) until the MMAs released every stage and Q
+      // used, the last commits that are issued.  (The last P V's own commit comes before that of its stage.)
       const uint64_t t0 = global_timer_ns();
       for (uint32_t j = issued > (uint32_t)STAGES ? issued - STAGES : 0; j < issued; ++j)
-        while (!mbar_try_wait(&gb->kv_full[j % STAGES], (j / STAGES) & 1u) && global_timer_ns() - t0 < BARRIER_LIMIT_NS) {}
+        while (!mbar_try_wait(&gb->kv_empty[j % STAGES], (j / STAGES) & 1u) && global_timer_ns() - t0 < BARRIER_LIMIT_NS) {}
       for (int t = 0; t < 2; ++t)
-        while (((q_used >> t) & 1u) && !mbar_try_wait(&gb->q_full[t], ((q_uses >> t) & 1u) ^ 1u) && global_timer_ns() - t0 < BARRIER_LIMIT_NS) {}
+        while (((q_used >> t) & 1u) && !mbar_try_wait(&gb->q_empty[t], ((q_uses >> t) & 1u) ^ 1u) && global_timer_ns() - t0 < BARRIER_LIMIT_NS) {}
     }
     __syncwarp();
   } else if (warp >= XA_MMA_WARP) {
