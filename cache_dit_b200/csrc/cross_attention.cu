@@ -129,7 +129,8 @@ __device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, const void*
                : "memory");
 }
 // tcgen05 instructions of a whole, converged warp: each elects its issuing lane itself (under a branch on an elected lane
-// the compiler spends many clocks making each operand uniform).
+// the compiler spends many clocks making each operand uniform).  Loads and stores of tensor memory (.aligned) are the whole
+// warp's too, so what depends on the lane is followed by __syncwarp() before them.
 #define CDB_XA_ELECTED(text) "{\n\t.reg .pred e, p;\n\telect.sync _|e, 0xffffffff;\n\t" text "\n\t}"
 __device__ __forceinline__ void xa_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(CDB_XA_ELECTED("setp.ne.b32 p, %4, 0;\n\t@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;")
@@ -399,10 +400,12 @@ __global__ void __launch_bounds__(XA_THREADS, 1) cross_attention_kernel(const __
           uint32_t o[16];
           tmem_ld_32x32b_x16(o_addr + c0, o);
           tmem_ld_wait();
-          if (out_row < 0) continue;
+          if (out_row >= 0) {
 #pragma unroll
-          for (int x = 0; x < 4; ++x)
-            if (c0 + 4 * x < p.d) *reinterpret_cast<uint4*>(dst + c0 + 4 * x) = make_uint4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
+            for (int x = 0; x < 4; ++x)
+              if (c0 + 4 * x < p.d) *reinterpret_cast<uint4*>(dst + c0 + 4 * x) = make_uint4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
+          }
+          __syncwarp();  // the next load from tensor memory is the whole warp's
         }
         if (out_row >= 0) p.part_ml[part_base + out_row] = make_float2(m == NEG_INF ? 0.f : m * p.c, l);
       } else {
@@ -435,6 +438,7 @@ __global__ void __launch_bounds__(XA_THREADS, 1) cross_attention_kernel(const __
           }
         }
       }
+      __syncwarp();
     };
     uint32_t posted = 0;
     // The tile's last P V is complete: its P may be overwritten, its O read.
@@ -460,6 +464,7 @@ __global__ void __launch_bounds__(XA_THREADS, 1) cross_attention_kernel(const __
             for (int x = 0; x < p.d; x += 8) *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + next_row * p.d + x) = make_uint4(0, 0, 0, 0);
           }
         }
+        __syncwarp();
         continue;
       }
       for (int j = 0; j < it.steps; ++j) {
@@ -495,6 +500,7 @@ __global__ void __launch_bounds__(XA_THREADS, 1) cross_attention_kernel(const __
                 for (int y = 0; y < 8; ++y) v_row[x * (XA_BOX_BYTES / 16) + y] = make_uint4(0, 0, 0, 0);
             }
             fence_async_smem();
+            __syncwarp();
           }
           at.next(STAGES);  // V
         }
@@ -502,6 +508,7 @@ __global__ void __launch_bounds__(XA_THREADS, 1) cross_attention_kernel(const __
         tcgen05_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&gb->s_turn[DP == 64 ? t : (t == 0 && it.tiles == 2 ? 1 : 0)]);  // the next scores may overwrite S
+        __syncwarp();
         if ((w.x & w.y & w.z & w.w) != 0xffffffffu) {
           const uint32_t word[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
@@ -563,6 +570,7 @@ __global__ void __launch_bounds__(XA_THREADS, 1) cross_attention_kernel(const __
             tcgen05_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&gb->p_full[t][q >> 1]);
+            __syncwarp();
           }
         }
         float l0, l1;
