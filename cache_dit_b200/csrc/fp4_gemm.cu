@@ -204,6 +204,7 @@ __device__ __forceinline__ void f4_store_block(const F4Params& p, uint8_t* block
     tma_store_2d(&p.map_out, block, n0 + c0, row0);
     bulk_commit_group();
   }
+  __syncwarp();  // what follows may be the whole warp's (a load from tensor memory, a barrier)
 }
 
 template <int CG, int BN, bool NV, typename T>
@@ -413,11 +414,13 @@ __global__ void __launch_bounds__(F4_THREADS, 1) fp4_gemm_kernel(const __grid_co
         s_col[c] = v;
       }
       ok = bounded_wait(&gb->acc_full[buf], (n_tile >> 1) & 1u, &gb->abort_flag, status_word, 25);
+      __syncwarp();
       ok = f4_epi_all(ok);  // publishes s_col, and makes the decision to go on the same in all its warps
       if (!ok) break;
       tcgen05_fence_after();
       const int row = row0 + lane;
       const float rs = row < p.M ? (p.ra != nullptr ? __ldg(p.ra + row) : 1.f) : 0.f;
+      __syncwarp();
       const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + buf * acc1;
       const bool live = row0 < p.M;  // warp-uniform: some of the 32 rows exist
       auto release = [&] {
@@ -427,6 +430,7 @@ __global__ void __launch_bounds__(F4_THREADS, 1) fp4_gemm_kernel(const __grid_co
           if constexpr (CG == 2) mbar_arrive_cluster(map_to_cta(smem_u32(&gb->acc_empty[buf]), 0));
           else mbar_arrive(&gb->acc_empty[buf]);
         }
+        __syncwarp();
       };
       auto plain_blocks = [&](int from, int to) {
 #pragma unroll 1
