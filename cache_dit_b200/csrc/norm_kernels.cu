@@ -150,6 +150,7 @@ __device__ __forceinline__ void fill8(float (&v)[8], float x) {
 // parity: a warp that is ahead writes other words than the ones a slower warp still reads, and cannot be two rows ahead.
 template <int TPR>
 __device__ __forceinline__ void row_barrier() {
+  __syncwarp();  // the barrier counts whole warps, and a lane that wrote a word may be apart
   asm volatile("bar.sync %0, %1;" ::"r"(1 + (int)threadIdx.x / TPR), "n"(TPR) : "memory");
 }
 template <int TPR>
