@@ -16,7 +16,9 @@
 //   * the output goes through shared memory and TMA: stores of a thread per row took 5500 clocks a tile;
 //   * O is rescaled only when a row's maximum has grown by more than 2^8: until then P simply grows to at most 2^8, which
 //     costs nothing in a floating type.  P is rounded to 16 bits for the product (a relative 2^-8 or 2^-11 each at most,
-//     averaged over the keys); m, l, S and O are fp32.
+//     averaged over the keys); m, l, S and O are fp32.  In fp16, P and l carry a factor of 2^7, the largest that keeps P
+//     below 2^16: weights under 2^-25 of the largest would round to zero, and thousands of them may stand beside one key
+//     that dominates.  With it a key loses 2^-32 of the largest at most.
 // Few rows over many keys: the key range is split over CTAs, partial (O, m, l) are joined by a second kernel.
 //
 // Warps: 0..3 and 4..7 the tiles' softmax and output, 8 TMA, 9 and 10 the tiles' products.
@@ -35,6 +37,7 @@ constexpr int XA_MAX_STAGES = 10;
 constexpr int XA_MAX_SPLIT = 64;
 constexpr int XA_MAX_GROUP = 32;  // heads of a tile
 constexpr float XA_LAZY = 8.0f;  // log2 of how far P may grow before O is rescaled
+constexpr float XA_F16_RAISE = 7.0f;  // log2 of the factor on P and l in fp16
 constexpr int XA_BOX_BYTES = 128 * 128;  // 128 rows x 64 elements
 constexpr int XA_WARP_BOX = XA_BOX_BYTES / 4;
 template <int DP>
@@ -548,7 +551,7 @@ __global__ void __launch_bounds__(XA_THREADS, 1) cross_attention_kernel(const __
           }
           tmem_st_wait();
         }
-        const float mc = m == NEG_INF ? 0.f : m * p.c;  // a row of -inf alone: P = 0
+        const float mc = m == NEG_INF ? 0.f : m * p.c - (BF16 ? 0.f : XA_F16_RAISE);  // a row of -inf alone: P = 0
         const uint64_t c2 = f32_pair(p.c, p.c), mc2 = f32_pair(-mc, -mc);
         uint64_t sum2[2] = {0, 0};
 #pragma unroll
