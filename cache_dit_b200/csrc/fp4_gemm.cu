@@ -171,11 +171,20 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   }
 }
 
+// The scale of an activation row in two factors, low <= 1 <= high (a NaN is in high).  An accumulator is in units of both
+// operands' scaled codes, up to 2^37: times a large row scale it may be beyond fp32 where the weight row's small scale would
+// bring it back, and the other way round with small ones.  low, then the weight's scale, then high: no step is larger than
+// the result, and none but the last smaller than 2^-120.
+struct RowScale {
+  float low, high;
+  __device__ __forceinline__ explicit RowScale(float s) : low(s < 1.f ? s : 1.f), high(s < 1.f ? 1.f : s) {}
+};
+
 // One staged block: 32 rows x 64 columns starting at local column `c0` of the tile, from 2 x 32 accumulator registers.
 template <typename T>
 __device__ __forceinline__ void f4_store_block(const F4Params& p, uint8_t* block,
                                                const uint32_t (&lo)[32], const uint32_t (&hi)[32], int c0, int n0,
-                                               int row0, float rs, const float2* s_col, int lane) {
+                                               int row0, const RowScale& rs, const float2* s_col, int lane) {
   if (n0 + c0 >= p.N) return;
   if (lane == 0) bulk_wait_group_read<0>();  // the store before this one is done reading
   __syncwarp();
@@ -189,7 +198,7 @@ __device__ __forceinline__ void f4_store_block(const F4Params& p, uint8_t* block
       const float4 sb = *reinterpret_cast<const float4*>(s_col + c0 + c);  // (scale, bias) of two columns
       const float a0 = __uint_as_float(c < 32 ? lo[c & 31] : hi[c & 31]);
       const float a1 = __uint_as_float(c < 32 ? lo[(c + 1) & 31] : hi[(c + 1) & 31]);
-      float v0 = fmaf(a0 * rs, sb.x, sb.y), v1 = fmaf(a1 * rs, sb.z, sb.w);
+      float v0 = fmaf(a0 * rs.low * sb.x, rs.high, sb.y), v1 = fmaf(a1 * rs.low * sb.z, rs.high, sb.w);
       if (p.gelu) {
         v0 = gelu_tanh(v0);
         v1 = gelu_tanh(v1);
@@ -419,7 +428,7 @@ __global__ void __launch_bounds__(F4_THREADS, 1) fp4_gemm_kernel(const __grid_co
       if (!ok) break;
       tcgen05_fence_after();
       const int row = row0 + lane;
-      const float rs = row < p.M ? (p.ra != nullptr ? __ldg(p.ra + row) : 1.f) : 0.f;
+      const RowScale rs(row < p.M && p.ra != nullptr ? __ldg(p.ra + row) : 1.f);
       __syncwarp();
       const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + buf * acc1;
       const bool live = row0 < p.M;  // warp-uniform: some of the 32 rows exist
@@ -605,7 +614,8 @@ __global__ void __launch_bounds__(F4V_THREADS, 4)
     const int n = n0 + 32 * j;
     if (lane == j && n < N) {
       const float cs = rw != nullptr ? __ldg(rw + n) : 1.f;
-      float v = fmaf(acc[j] * (ra != nullptr ? __ldg(ra) : 1.f), cs, bias != nullptr ? (float)bias[n] : 0.f);
+      const RowScale rs(ra != nullptr ? __ldg(ra) : 1.f);
+      float v = fmaf(acc[j] * rs.low * cs, rs.high, bias != nullptr ? (float)bias[n] : 0.f);
       if (gelu) v = gelu_tanh(v);
       out[n] = (T)v;
     }
