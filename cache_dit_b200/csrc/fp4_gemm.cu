@@ -548,6 +548,10 @@ __global__ void __launch_bounds__(F4V_THREADS, 4)
       s_a[j * chunks + c] = make_uint4(f[0], f[1], f[2], f[3]);
     }
     s_s[c] = chunk_scales<NV>(*reinterpret_cast<const uint32_t*>(a_scales + fp4_scale_word(0, c >> PER_WORD, tiles)), c);
+    if constexpr (!NV) {  // one scale for the 32 columns, 2^-127 .. 2^127: in two factors, as a row scale
+      const RowScale s(s_s[c].x);
+      s_s[c] = make_float2(s.low, s.high);
+    }
   }
   __syncthreads();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -590,7 +594,8 @@ __global__ void __launch_bounds__(F4V_THREADS, 4)
         t = __hfma2(h2(f1[2]), h2(av[2 * b + 1].z), t);
         t = __hfma2(h2(f1[3]), h2(av[2 * b + 1].w), t);
         const float2 d = __half22float2(t);
-        acc[j] = fmaf(d.x + d.y, b ? ws.y * as.y : ws.x * as.x, acc[j]);
+        if constexpr (NV) acc[j] = fmaf(d.x + d.y, b ? ws.y * as.y : ws.x * as.x, acc[j]);
+        else acc[j] = fmaf((d.x + d.y) * as.x * ws.x, as.y, acc[j]);  // the scales' product alone may be beyond fp32
       }
     }
   }

@@ -47,3 +47,14 @@ def test_one_loud_element(fmt, m):
   w = torch.full((136, 64), 1e-3)
   w[:, 32:] = 2.0
   _compare(a.to(torch.bfloat16), w.to(torch.bfloat16), fmt)
+
+
+@pytest.mark.parametrize("m", [1, 3, 130])
+def test_block_scales_whose_product_is_beyond_fp32(m):
+  """mxfp4 blocks of 2^98 and 2^30: their scales' product is 2^128, their sums of codes 0.25 and 0."""
+  a, w = torch.zeros(m, 64), torch.zeros(24, 64)
+  a[:, 0], a[:, 1] = 2.0**97, 2.0**100
+  w[:, 0], w[:, 2] = 2.0**29, 2.0**32
+  _compare(a.to(torch.bfloat16), w.to(torch.bfloat16), "mxfp4")
+  w[:, 0] = 0.0
+  _compare(a.to(torch.bfloat16), w.to(torch.bfloat16), "mxfp4")
