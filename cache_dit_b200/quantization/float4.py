@@ -219,7 +219,8 @@ def float4_linear(x: torch.Tensor, w: Float4Rows, bias: Optional[torch.Tensor] =
 
 class Float4Linear(torch.nn.Module):
   """y = float4_linear(x, W): an nn.Linear replacement with 4-bit activations and weights, bfloat16 in and out.  The weight
-  is quantised once; codes and scales are buffers, so they move and save with the module."""
+  is quantised once; codes and scales are buffers, so they move and save with the module.  A cast of the module (`.half()`,
+  `.to(dtype)`) leaves them and the bias in their types."""
 
   def __init__(self, weight: Float4Rows, bias: Optional[torch.Tensor]):
     super().__init__()
@@ -245,6 +246,16 @@ class Float4Linear(torch.nn.Module):
   def supports(linear: torch.nn.Linear) -> bool:
     n, k = linear.weight.shape
     return linear.weight.dtype == torch.bfloat16 and k % 32 == 0 and 0 < k <= _native.FP4_MAX_COLS and n % 8 == 0 and n > 0
+
+  def _apply(self, fn, recurse: bool = True):
+    """`.to()`, `.half()` and the like: the buffers follow the device, their types are the kernels' and stay."""
+    before = dict(self._buffers)
+    super()._apply(fn, recurse)
+    for name, old in before.items():
+      new = self._buffers[name]
+      if old is not None and new.dtype != old.dtype:
+        self._buffers[name] = old.to(new.device)
+    return self
 
   @property
   def weight_rows(self) -> Float4Rows:
