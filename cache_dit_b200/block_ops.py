@@ -2,8 +2,8 @@
 encoder's states.
 
 In the models the reference wraps these are eager PyTorch ops inside the diffusers blocks.  Inference only: inputs that
-ask for gradients are refused.  All tensors of a call lie on one CUDA device; results are new, contiguous tensors on the
-current stream of that device.
+carry a derivative (backward or forward mode) are refused.  All tensors of a call lie on one CUDA device; results are new,
+contiguous tensors on the current stream of that device.
 """
 from __future__ import annotations
 

@@ -7,7 +7,7 @@ Two formats, both of e2m1 codes (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign):
   "mxfp4"  blocks of 32 with a power-of-two scale (OCP microscaling).
 The arithmetic and the layout of the scales are those of `cdb_fp4_quant_rows` in include/cache_dit_b200.h.
 
-Inference only: none of these has a backward pass, and inputs that ask for one are refused.
+Inference only: none of these has a backward pass or a forward-mode derivative, and inputs that carry one are refused.
 """
 from __future__ import annotations
 
@@ -15,6 +15,7 @@ import dataclasses
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _native
 
@@ -66,10 +67,18 @@ def _check_cols(cols: int) -> None:
 
 
 def refuse(what: str, *tensors) -> None:
-  """Checks every operator here makes of its tensors (None: absent): all on one CUDA device, and none that asks for a
-  gradient, which would be lost silently (no backward pass)."""
+  """Checks every operator here makes of its tensors (None: absent): none that carries a derivative, which would be lost
+  silently (there is no backward pass and no forward-mode rule), and all on one CUDA device."""
+  forward = forward_ad._current_level >= 0  # no_grad does not end forward mode
+  if forward or torch.is_grad_enabled():
+    for t in tensors:
+      if t is None:
+        continue
+      if t.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad() or on detached tensors")
+      if forward and forward_ad.unpack_dual(t).tangent is not None:
+        raise RuntimeError(f"{what} has no forward-mode derivative: call it on the primal tensors (forward_ad.unpack_dual)")
   device = None
-  grad = torch.is_grad_enabled()
   for t in tensors:
     if t is None:
       continue
@@ -80,8 +89,6 @@ def refuse(what: str, *tensors) -> None:
     elif t.device != device:
       _native._need_cuda(t)
       raise RuntimeError(f"{what}: all tensors must be on one device")
-    if grad and t.requires_grad:
-      raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad() or on detached tensors")
 
 
 def _check_rows(t: Float4Rows, what: str) -> int:
