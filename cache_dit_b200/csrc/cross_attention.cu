@@ -806,7 +806,7 @@ extern "C" int cdb_cross_attention(const void* q_v, const void* k_v, const void*
   if (sq > INT32_MAX - 256 || skv > INT32_MAX - 256 || heads > 65535 || batch > INT32_MAX) return CDB_ERR_TOO_LARGE;
   const int sms = sm_count();
   const XaPlan plan = xa_plan(batch, sq, skv, heads, kv_heads, d, key_mask != nullptr, sms);
-  if (plan.items > INT32_MAX) return CDB_ERR_TOO_LARGE;
+  if (plan.items > INT32_MAX - sms) return CDB_ERR_TOO_LARGE;  // a block's item index goes a grid's step past the last
   if (plan.bytes > workspace_bytes || (plan.bytes > 0 && !workspace)) return CDB_ERR_SCRATCH_TOO_SMALL;
   if (!aligned16(workspace)) return CDB_ERR_UNSUPPORTED;
   const bool bf16 = dtype == CDB_BF16;
