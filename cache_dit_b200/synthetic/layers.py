@@ -92,15 +92,18 @@ def gated_add_layer_norm_linear(x: torch.Tensor, gate: torch.Tensor, y: torch.Te
 
 def encoder_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, key_mask: Optional[torch.Tensor] = None) -> torch.Tensor:
   """Attention of q [B, S, H, D] to an encoder's k, v [B, T, H, D]; key_mask bool [B, T] names the tokens of each prompt
-  (a batch of prompts padded to one length).  Masked prompts go through this package's kernel on the GPU; without a mask
-  the library's attention runs, as it does for self-attention."""
+  (a batch of prompts padded to one length).  Masked prompts go through this package's kernel on the GPU (16-bit types, heads
+  of a multiple of 8 up to 128; anything else in plain form); without a mask the library's attention runs, as it does for
+  self-attention."""
   if key_mask is None:
     return F.scaled_dot_product_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2)).transpose(1, 2)
-  if q.is_cuda and q.dtype in (torch.bfloat16, torch.float16) and not torch.is_grad_enabled():
+  d = q.shape[-1]
+  if q.is_cuda and q.dtype in (torch.bfloat16, torch.float16) and d % 8 == 0 and d <= _native.CROSS_MAX_HEAD_DIM and \
+      not torch.is_grad_enabled():
     return cross_attention(q, k, v, key_mask)
   keep = key_mask[:, None, None, :]
   v = torch.where(key_mask[:, :, None, None], v, torch.zeros_like(v))
-  scores = (q.transpose(1, 2).float() @ k.permute(0, 2, 3, 1).float()) * q.shape[-1]**-0.5
+  scores = (q.transpose(1, 2).float() @ k.permute(0, 2, 3, 1).float()) * d**-0.5
   p = torch.softmax(scores.masked_fill(~keep, float("-inf")), dim=-1)
   p = torch.where(keep.any(dim=-1, keepdim=True), p, torch.zeros_like(p)).to(v.dtype)  # a prompt without tokens: zeros
   return (p @ v.transpose(1, 2)).transpose(1, 2)
