@@ -685,8 +685,11 @@ def _status_ptr(index: int) -> int:
 
 
 def _on_device(index: int, fn, what: str, *args):
-  """fn(*args, stream) with the tensors' device current, on its current stream."""
+  """fn(*args, stream) with the tensors' device current, on its current stream.  Whatever the first call on a device is, it
+  makes the mailbox, so that a product or attention whose own first call is captured finds a status word."""
   global launch_count
+  if index not in _status_ptrs:
+    _status_ptr(index)
   if index == _current_device():
     st = fn(*args, _raw_stream(index))
   else:

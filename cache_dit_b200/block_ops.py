@@ -3,7 +3,9 @@ encoder's states.
 
 In the models the reference wraps these are eager PyTorch ops inside the diffusers blocks.  Inference only: inputs that
 carry a derivative (backward or forward mode) are refused.  All tensors of a call lie on one CUDA device; results are new,
-contiguous tensors on the current stream of that device.
+contiguous tensors on the current stream of that device.  A wait inside the attention that runs out leaves its output
+incomplete and is latched in the device's status word: the cache engine raises it at its next step, a direct caller asks
+`_native.check_device_status(device)`.
 """
 from __future__ import annotations
 

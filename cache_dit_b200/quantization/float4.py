@@ -8,6 +8,8 @@ Two formats, both of e2m1 codes (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign):
 The arithmetic and the layout of the scales are those of `cdb_fp4_quant_rows` in include/cache_dit_b200.h.
 
 Inference only: none of these has a backward pass or a forward-mode derivative, and inputs that carry one are refused.
+A wait inside the product that runs out leaves its output incomplete and is latched in the device's status word: the cache
+engine raises it at its next step, a direct caller asks `_native.check_device_status(device)`.
 """
 from __future__ import annotations
 
