@@ -5,9 +5,10 @@
 // Codes are e2m1 (sign, 0 0.5 1 1.5 2 3 4 6), the even element in the low half of a byte.
 //
 // Why the row scale is a power of two: every decision is then exact.  A block's scale is e4m3(max / 6 / 2^p) and a
-// code is the e2m1 number nearest to x / (scale * 2^p), i.e. quotients of a 16-bit number by a number of at most
-// four bits.  Such a quotient lies on a rounding boundary exactly or misses it by more than 2^-12, so a quotient
-// rounded once to fp32 decides like the infinitely precise one.  e4m3 is a floating format: the up to one bit of its
+// code is the e2m1 number nearest to x / (scale * 2^p), i.e. quotients of x by a number of at most four bits.  A boundary
+// times that number has at most seven bits: an x that is not on it is at least one of its last places away, and the
+// quotient more than half a last place of the boundary.  So a quotient rounded once to fp32 decides like the infinitely
+// precise one, for fp32 rows as for 16-bit ones.  e4m3 is a floating format: the up to one bit of its
 // range that a power of two leaves unused costs no precision.
 //
 // Block scales lie as the tensor core reads them: tiles of 128 rows x 4 scales = 512 bytes, byte
@@ -88,8 +89,8 @@ __device__ __forceinline__ float fp4_row_scale(float top) {
 
 // The scale byte of a block whose largest magnitude is `top`, and how its elements become codes:
 // code = e2m1(q), q = x / step.  nvfp4: q from an approximate reciprocal and one correction, q' = q + (x - q step) inverse:
-// a quotient that is an fp32 number (a rounding boundary is) comes out as that number, any other within a last place,
-// which is all that a decision needs; mxfp4: step is a power of two, x * inverse is exact.
+// the residual is exact and the correction good to 2^-40, while the quotient of an fp32 number by one of four bits is no
+// nearer than 1/30 of a last place to the middle of two fp32 numbers: q' is the nearest fp32 number; mxfp4: step is a power of two, x * inverse is exact.
 struct Fp4Step {
   uint32_t byte;
   float step, inverse;
