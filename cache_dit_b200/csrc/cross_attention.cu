@@ -695,9 +695,12 @@ struct XaPlan {
 static size_t xa_round(size_t n) { return (n + 255) / 256 * 256; }
 
 // Heads of a tile: the largest power of two up to 32 that divides the group, so that 32 rows, a warp's, are whole
-// queries of all of them.  Splits of the key range: items cost their
-// steps plus about four more for their first loads and their output, a split launch about four for the join; the number
-// of splits is the one whose waves over the SMs cost least.
+// queries of all of them.  Splits of the key range: items cost their steps plus about four more for their first loads
+// and their output; a split launch about four for the join, and the time its fp32 partials take to HBM and back, a step
+// (1.4 to 1.6 us) for 8.5 MB.  The number of splits is the one whose waves over the SMs cost least.  Measured, unsplit
+// against the best split: 1 x 6400 x 4096, 12 heads of 128 175 : 218 us (2 parts), 1 x 1024 x 4096 x 24 65 : 75 (3),
+// 1 x 256 x 1024 x 40 20 : 25 (2), 1 x 300 x 4096 x 24 59 : 37 (3), 1 x 2560 x 8192 x 15 224 : 206 (3; 2 and 4 parts 208
+// and 210), one query on 16385 keys, 4 x 32 heads on 8 key heads 193 : 59 (4).
 static XaPlan xa_plan(int64_t batch, int64_t sq, int64_t skv, int64_t heads, int64_t kv_heads, int64_t d, bool masked, int sms) {
   XaPlan p{};
   const int group = (int)(heads / kv_heads);
@@ -712,7 +715,8 @@ static XaPlan xa_plan(int64_t batch, int64_t sq, int64_t skv, int64_t heads, int
   double best = 1e300;
   for (int n = 1; n <= XA_MAX_SPLIT && n <= p.key_tiles; ++n) {
     const int64_t waves = (items * n + sms - 1) / sms;
-    const double cost = (double)waves * ((p.key_tiles + n - 1) / n + 4) + (n > 1 ? 4 : 0);
+    const double partials = n > 1 ? 2.0 * n * (double)p.rows * (double)(d * 4 + 8) : 0.0;  // bytes, written and read
+    const double cost = (double)waves * ((p.key_tiles + n - 1) / n + 4) + (n > 1 ? 4 : 0) + partials / 8.5e6;
     if (cost < best) {
       best = cost;
       p.splits = n;
